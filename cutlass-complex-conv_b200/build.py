@@ -6,7 +6,7 @@ Produces, next to the Python sources in ``complex_conv2d/``:
   * ``libccv_b200.so`` - the CUDA kernels and the C ABI (include/ccv_b200.h),
     compiled by nvcc for sm_100a only (no torch dependency);
   * ``_C.so``          - the torch/pybind extension ``complex_conv2d._C``
-    (csrc/bindings.cpp), linked against libccv_b200.so with an $ORIGIN rpath.
+    (csrc/bindings*.cpp), linked against libccv_b200.so with an $ORIGIN rpath.
 
 Both are cross-compiled here without a GPU; nothing is JIT-built at import
 time.  Each CUDA translation unit compiles to an object under ``_build/`` in
@@ -29,9 +29,11 @@ INCLUDE = os.path.join(REPO, "include")
 OBJ = os.path.join(HERE, "_build")
 
 CU_SOURCES = ["ccv_api.cu", "ccv_fprop.cu", "ccv_fprop2.cu", "ccv_fprop2h.cu", "ccv_layout.cu",
-              "ccv_noalloc.cu", "ccv_backward.cu"]
+              "ccv_noalloc.cu", "ccv_backward.cu", "ccv_norm.cu", "ccv_ffn.cu", "ccv_dropout.cu",
+              "ccv_tokens_api.cu"]
 CU_HEADERS = ["ccv_internal.h", "ccv_ptx.cuh", "ccv_fprop_common.cuh", "ccv_epilogue.cuh",
-              "ccv_layout_role.cuh"]
+              "ccv_layout_role.cuh", "ccv_tokens.cuh"]
+EXT_SOURCES = ["bindings.cpp", "bindings_tokens.cpp"]
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -81,12 +83,13 @@ def build_ext(verbose: bool = False, force: bool = False) -> str:
 
     lib = build_lib(verbose, force)
     out = os.path.join(PKG, "_C.so")
-    src = os.path.join(CSRC, "bindings.cpp")
-    if force or _stale(out, [src, lib, os.path.join(INCLUDE, "ccv_b200.h")]):
-        incs = ce.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE]
+    srcs = [os.path.join(CSRC, f) for f in EXT_SOURCES]
+    if force or _stale(out, [*srcs, os.path.join(CSRC, "bindings_tokens.h"), lib,
+                             os.path.join(INCLUDE, "ccv_b200.h")]):
+        incs = ce.include_paths("cuda") + [sysconfig.get_paths()["include"], INCLUDE, CSRC]
         libdirs = ce.library_paths("cuda")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src,
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *srcs,
                f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
                "-DTORCH_API_INCLUDE_EXTENSION_H", "-w"]
         for i in incs:

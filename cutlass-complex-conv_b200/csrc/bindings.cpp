@@ -15,6 +15,7 @@
 #include <string>
 #include <vector>
 
+#include "bindings_tokens.h"
 #include "ccv_b200.h"
 
 namespace {
@@ -539,6 +540,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("x"), pybind11::arg("dy"), pybind11::arg("kernel_h"),
         pybind11::arg("kernel_w"), pybind11::arg("stride_h"), pybind11::arg("stride_w"),
         pybind11::arg("pad_h"), pybind11::arg("pad_w"));
+  register_token_operators(m);
   m.def("device_status", &device_status, pybind11::arg("device"));
   m.def("clear_device_status", &clear_device_status, pybind11::arg("device"));
   m.def("selftest_bounded_wait", &selftest_bounded_wait, pybind11::arg("device"),

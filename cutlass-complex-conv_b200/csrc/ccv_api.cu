@@ -307,6 +307,12 @@ int check_status_clear() {
 
 }  // namespace
 
+int begin_launches(cudaStream_t stream) {
+  ensure_status_mirror(stream);
+  const int rc = check_device();
+  return rc != CCV_OK ? rc : check_status_clear();
+}
+
 int device_sm_count() {
   int dev = 0;
   if (current_device(&dev) != CCV_OK) return 148;

@@ -1,0 +1,97 @@
+// Dropout from a counter-based generator, with an optional residual added.
+//
+// Element i of a call with key `seed` and stream `offset` takes 16 bits of
+// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", 2011) at counter (i / 8, offset): eight
+// 16-bit parts per evaluation, low half of each word first.  It is dropped
+// when its part is below t = round(p 65536), else scaled by 65536/(65536-t),
+// the inverse of the share kept exactly, so the expectation is unbiased.
+// The mask is a function of (seed, offset, i): the backward pass is the same
+// call on the gradient, and nothing is stored.
+#include <cmath>
+
+#include "ccv_internal.h"
+#include "ccv_ptx.cuh"
+#include "ccv_tokens.cuh"
+
+namespace ccv {
+
+namespace {
+
+__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = static_cast<uint64_t>(c.x) * 0xD2511F53u;
+    const uint64_t b = static_cast<uint64_t>(c.z) * 0xCD9E8D57u;
+    c = make_uint4(static_cast<uint32_t>(b >> 32) ^ c.y ^ k.x, static_cast<uint32_t>(b),
+                   static_cast<uint32_t>(a >> 32) ^ c.w ^ k.y, static_cast<uint32_t>(a));
+    k.x += 0x9E3779B9u;
+    k.y += 0xBB67AE85u;
+  }
+  return c;
+}
+
+// One thread per group of eight elements.
+template <typename Tx, typename Tr>
+__global__ void dropout_groups(const Tx* __restrict__ x, const Tr* __restrict__ residual,
+                               Tr* __restrict__ y, int64_t count, uint32_t threshold, float scale,
+                               uint64_t seed, uint64_t offset,
+                               const int64_t* __restrict__ offset_dev) {
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  if (offset_dev != nullptr) offset = static_cast<uint64_t>(*offset_dev);
+  const uint2 key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
+  const int64_t groups = (count + 7) / 8;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups;
+       g += step) {
+    const uint4 r = philox4x32_10(
+        make_uint4(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32),
+                   static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
+        key);
+    const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t i = g * 8 + j;
+      if (i < count) {
+        const uint32_t part = (word[j / 2] >> (16 * (j & 1))) & 0xffffu;
+        float v = part >= threshold ? to_f32(x[i]) * scale : 0.f;
+        if (residual != nullptr) v += to_f32(residual[i]);
+        y[i] = from_f32<Tr>(v);
+      }
+    }
+  }
+}
+
+template <typename Tx, typename Tr>
+int run_dropout(const Dropout& a, cudaStream_t stream) {
+  const uint32_t threshold = static_cast<uint32_t>(std::floor(a.p * 65536.0 + 0.5));
+  const float scale =
+      threshold >= 65536u ? 0.f : static_cast<float>(65536.0 / (65536.0 - threshold));
+  const int64_t blocks64 = ((a.count + 7) / 8 + 255) / 256;
+  const unsigned blocks = static_cast<unsigned>(blocks64 < 148 * 16 ? blocks64 : 148 * 16);
+  return launched(
+      launch_kernel(dropout_groups<Tx, Tr>, dim3(blocks), dim3(256), 0, stream, 1,
+                    static_cast<const Tx*>(a.x), static_cast<const Tr*>(a.residual),
+                    static_cast<Tr*>(a.y), a.count, threshold, scale, a.seed, a.offset,
+                    a.offset_dev),
+      "dropout");
+}
+
+}  // namespace
+
+int launch_dropout(const Dropout& a, cudaStream_t stream) {
+  if (a.x_dtype == CCV_DTYPE_BF16) {
+    return a.y_dtype == CCV_DTYPE_F32 ? run_dropout<__nv_bfloat16, float>(a, stream)
+                                      : run_dropout<__nv_bfloat16, __nv_bfloat16>(a, stream);
+  }
+  if (a.x_dtype == CCV_DTYPE_F16) {
+    return a.y_dtype == CCV_DTYPE_F32 ? run_dropout<__half, float>(a, stream)
+                                      : run_dropout<__half, __half>(a, stream);
+  }
+  if (a.y_dtype == CCV_DTYPE_BF16) return run_dropout<float, __nv_bfloat16>(a, stream);
+  if (a.y_dtype == CCV_DTYPE_F16) return run_dropout<float, __half>(a, stream);
+  return run_dropout<float, float>(a, stream);
+}
+
+}  // namespace ccv

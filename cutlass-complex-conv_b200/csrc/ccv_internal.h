@@ -17,6 +17,15 @@ int set_error(int code, const std::string& msg);
 // Converts a CUDA runtime error into CCV_ERR_CUDA with context.
 int cuda_error(cudaError_t e, const char* what);
 
+// CCV_OK for a launch that succeeded, cuda_error() otherwise.
+inline int launched(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? CCV_OK : cuda_error(e, what);
+}
+
+// What every launching entry point does after its argument checks: sets up
+// the status mirror, requires an sm_100 device and a clear status.
+int begin_launches(cudaStream_t stream);
+
 // Device pointer of the per-device status word (the current device).
 int* device_status_ptr();
 
@@ -162,6 +171,73 @@ int launch_dgrad_phase_pad_planar(const float* dy_r, const float* dy_i, float* o
                                   cudaStream_t stream);
 int launch_dgrad_interleave_planar(const float* phases, float* dx_r, float* dx_i, const Problem& pb,
                                    cudaStream_t stream);
+
+// Token operators (ccv_norm.cu, ccv_ffn.cu, ccv_dropout.cu).  Arguments are
+// checked by the entry points (ccv_tokens_api.cu); row strides in elements.
+struct NormForward {
+  const void* x;
+  int64_t x_stride;
+  const void *weight, *bias;  // either may be null
+  float eps;
+  void* y;                    // dense
+  float *mean, *rstd;         // either may be null
+  int64_t rows, features;
+  int x_dtype, weight_dtype, y_dtype;
+};
+int launch_norm_forward(const NormForward& a, cudaStream_t stream);
+struct NormBackward {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const float *mean, *rstd;
+  const void* weight;           // may be null
+  void *dx, *dweight, *dbias;   // dense; each may be null
+  int64_t rows, features;
+  int x_dtype, weight_dtype, y_dtype;
+};
+size_t norm_backward_workspace_bytes(int64_t rows, int64_t features);
+int launch_norm_backward(const NormBackward& a, void* ws, cudaStream_t stream);
+
+struct FfnShape {
+  int64_t rows, features, hidden;
+  int dtype, activation;
+};
+struct FfnForward {
+  FfnShape shape;
+  const void* x;
+  int64_t x_stride;
+  const void *w_gate, *w_up, *w_down;
+  void* y;
+  void* saved;  // h, g, u planes for the backward pass, or null
+};
+struct FfnBackward {
+  FfnShape shape;
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const void *w_gate, *w_up, *w_down, *saved;
+  void *dx, *dw_gate, *dw_up, *dw_down;  // each may be null
+};
+// Bytes of one [rows][hidden] plane (rows padded to 16 bytes).
+size_t ffn_plane_bytes(const FfnShape& s);
+size_t ffn_forward_workspace_bytes(const FfnShape& s);
+size_t ffn_backward_workspace_bytes(const FfnShape& s);
+int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream);
+int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream);
+
+struct Dropout {
+  const void* x;
+  const void* residual;  // may be null; of y's type
+  void* y;
+  int64_t count;
+  int x_dtype, y_dtype;
+  double p;
+  uint64_t seed, offset;
+  const int64_t* offset_dev;  // overrides offset when not null
+};
+int launch_dropout(const Dropout& a, cudaStream_t stream);
 
 // Encodes a tiled tensor map through the driver entry point.
 // `swizzle_bytes` is 64 or 128 (the box's inner extent in bytes).

@@ -1,0 +1,260 @@
+// extern "C" entry points of the token operators (declared in
+// include/ccv_b200.h): argument checks, then the launchers.  No C++ exception
+// leaves them.
+#include <cmath>
+#include <exception>
+
+#include "ccv_internal.h"
+#include "ccv_tokens.cuh"
+
+namespace ccv {
+namespace {
+
+// Runs body(), turning an exception (an allocation of an error text) into a
+// status.
+template <typename Fn>
+int guarded(Fn&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return CCV_ERR_CUDA;
+  }
+}
+
+int invalid(const char* msg) { return set_error(CCV_ERR_INVALID_ARGUMENT, msg); }
+
+bool aligned_to(const void* p, size_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+constexpr int64_t kMaxExtent = 0x7fffffffLL;
+constexpr int64_t kMaxElements = 1LL << 40;
+
+int check_rows(int64_t rows, int64_t features) {
+  if (rows < 0) return invalid("rows must be non-negative");
+  if (features <= 0) return invalid("features must be positive");
+  if (rows > kMaxExtent || features > kMaxExtent || rows * features > kMaxElements) {
+    return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
+  }
+  return CCV_OK;
+}
+
+int check_norm_types(int x_dtype, int weight_dtype, int y_dtype) {
+  if (!valid_dtype(x_dtype) || !valid_dtype(weight_dtype) || !valid_dtype(y_dtype)) {
+    return invalid("unknown element type");
+  }
+  if (weight_dtype != CCV_DTYPE_F32 && weight_dtype != x_dtype) {
+    return invalid("layer norm weights must be float32 or of the input's type");
+  }
+  if (x_dtype != CCV_DTYPE_F32 && y_dtype != CCV_DTYPE_F32 && y_dtype != x_dtype) {
+    return invalid("a 16-bit input gives an output of its own type or float32");
+  }
+  return CCV_OK;
+}
+
+int check_ffn(const FfnShape& s) {
+  if (s.dtype != CCV_DTYPE_BF16 && s.dtype != CCV_DTYPE_F16) {
+    return invalid("the gated feed-forward block takes bfloat16 or float16");
+  }
+  if (s.activation != CCV_ACTIVATION_SILU && s.activation != CCV_ACTIVATION_GELU) {
+    return invalid("unknown activation");
+  }
+  if (s.hidden <= 0) return invalid("hidden must be positive");
+  int rc = check_rows(s.rows, s.features);
+  if (rc == CCV_OK) rc = check_rows(s.rows, s.hidden);
+  if (rc == CCV_OK) rc = check_rows(s.hidden, s.features);
+  return rc;
+}
+
+int check_workspace(const void* ws, size_t have, size_t need) {
+  if (need == 0) return CCV_OK;
+  if (ws == nullptr || !aligned_to(ws, 256) || have < need) {
+    return set_error(CCV_ERR_WORKSPACE, "workspace missing, misaligned or too small");
+  }
+  return CCV_OK;
+}
+
+}  // namespace
+}  // namespace ccv
+
+using namespace ccv;
+
+extern "C" {
+
+int ccv_layer_norm_forward(const void* x, int x_dtype, int64_t x_row_stride, const void* weight,
+                           const void* bias, int weight_dtype, float eps, void* y, int y_dtype,
+                           float* mean, float* rstd, int64_t rows, int64_t features,
+                           ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    int rc = check_rows(rows, features);
+    if (rc == CCV_OK) rc = check_norm_types(x_dtype, weight_dtype, y_dtype);
+    if (rc != CCV_OK) return rc;
+    if (!(eps >= 0.f) || std::isinf(eps)) return invalid("eps must be non-negative and finite");
+    if (rows == 0) return CCV_OK;
+    if (x == nullptr || y == nullptr) return invalid("null tensor pointer");
+    if (x_row_stride < 0) return invalid("row stride must be non-negative");
+    if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(y, dtype_bytes(y_dtype)) ||
+        !aligned_to(weight, dtype_bytes(weight_dtype)) ||
+        !aligned_to(bias, dtype_bytes(weight_dtype)) || !aligned_to(mean, 4) ||
+        !aligned_to(rstd, 4)) {
+      return invalid("tensor pointers must be aligned to their element");
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = begin_launches(st)) != CCV_OK) return rc;
+    NormForward a = {x,    x_row_stride, weight,  bias,         eps,    y, mean, rstd, rows,
+                     features, x_dtype,  weight_dtype, y_dtype};
+    return launch_norm_forward(a, st);
+  });
+}
+
+size_t ccv_layer_norm_backward_workspace_bytes(int64_t rows, int64_t features) {
+  if (rows < 0 || features <= 0 || rows > kMaxExtent || features > kMaxExtent) return 0;
+  return norm_backward_workspace_bytes(rows, features);
+}
+
+int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, const void* x,
+                            int x_dtype, int64_t x_row_stride, const float* mean,
+                            const float* rstd, const void* weight, int weight_dtype, void* dx,
+                            void* dweight, void* dbias, int64_t rows, int64_t features,
+                            void* workspace, size_t workspace_bytes, ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    int rc = check_rows(rows, features);
+    if (rc == CCV_OK) rc = check_norm_types(x_dtype, weight_dtype, y_dtype);
+    if (rc != CCV_OK) return rc;
+    if (dx == nullptr && dweight == nullptr && dbias == nullptr) return CCV_OK;
+    if (rows > 0 && (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr)) {
+      return invalid("null tensor pointer");
+    }
+    if (x_row_stride < 0 || dy_row_stride < 0) return invalid("row stride must be non-negative");
+    if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(dx, dtype_bytes(x_dtype)) ||
+        !aligned_to(dy, dtype_bytes(y_dtype)) || !aligned_to(weight, dtype_bytes(weight_dtype)) ||
+        !aligned_to(dweight, dtype_bytes(weight_dtype)) ||
+        !aligned_to(dbias, dtype_bytes(weight_dtype)) || !aligned_to(mean, 4) ||
+        !aligned_to(rstd, 4)) {
+      return invalid("tensor pointers must be aligned to their element");
+    }
+    if ((rc = check_workspace(workspace, workspace_bytes,
+                              norm_backward_workspace_bytes(rows, features))) != CCV_OK) {
+      return rc;
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = begin_launches(st)) != CCV_OK) return rc;
+    NormBackward a = {dy, dy_row_stride, x,     x_row_stride, mean,     rstd,    weight,      dx,
+                      dweight, dbias,    rows,  features,     x_dtype,  weight_dtype, y_dtype};
+    return launch_norm_backward(a, workspace, st);
+  });
+}
+
+size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden) {
+  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
+  return 3 * ffn_plane_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+}
+
+size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden) {
+  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
+  return ffn_forward_workspace_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+}
+
+size_t ccv_gated_ffn_backward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden) {
+  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
+  return ffn_backward_workspace_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+}
+
+int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gate,
+                          const void* w_up, const void* w_down, void* y, int dtype,
+                          int activation, int64_t rows, int64_t features, int64_t hidden,
+                          void* saved, size_t saved_bytes, void* workspace,
+                          size_t workspace_bytes, ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    FfnForward f = {{rows, features, hidden, dtype, activation}, x,      x_row_stride, w_gate, w_up,
+                    w_down,                                      y, saved};
+    int rc = check_ffn(f.shape);
+    if (rc != CCV_OK || rows == 0) return rc;
+    if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr ||
+        y == nullptr) {
+      return invalid("null tensor pointer");
+    }
+    if (x_row_stride < 0) return invalid("row stride must be non-negative");
+    for (const void* p : {x, w_gate, w_up, w_down, static_cast<const void*>(y)}) {
+      if (!aligned_to(p, 2)) return invalid("tensor pointers must be aligned to their element");
+    }
+    if (saved != nullptr && (!aligned_to(saved, 256) || saved_bytes < 3 * ffn_plane_bytes(f.shape))) {
+      return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");
+    }
+    if ((rc = check_workspace(workspace, workspace_bytes,
+                              ffn_forward_workspace_bytes(f.shape))) != CCV_OK) {
+      return rc;
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = begin_launches(st)) != CCV_OK) return rc;
+    return launch_ffn_forward(f, workspace, st);
+  });
+}
+
+int ccv_gated_ffn_backward(const void* dy, int64_t dy_row_stride, const void* x,
+                           int64_t x_row_stride, const void* w_gate, const void* w_up,
+                           const void* w_down, const void* saved, size_t saved_bytes, void* dx,
+                           void* dw_gate, void* dw_up, void* dw_down, int dtype, int activation,
+                           int64_t rows, int64_t features, int64_t hidden, void* workspace,
+                           size_t workspace_bytes, ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    FfnBackward b = {{rows, features, hidden, dtype, activation},
+                     dy, dy_row_stride, x, x_row_stride, w_gate, w_up, w_down, saved,
+                     dx, dw_gate, dw_up, dw_down};
+    int rc = check_ffn(b.shape);
+    if (rc != CCV_OK) return rc;
+    if (dx == nullptr && dw_gate == nullptr && dw_up == nullptr && dw_down == nullptr) {
+      return CCV_OK;
+    }
+    if (w_gate == nullptr || w_up == nullptr || w_down == nullptr ||
+        (rows > 0 && (dy == nullptr || x == nullptr || saved == nullptr))) {
+      return invalid("null tensor pointer");
+    }
+    if (x_row_stride < 0 || dy_row_stride < 0) return invalid("row stride must be non-negative");
+    for (const void* p : {dy, x, w_gate, w_up, w_down, static_cast<const void*>(dx),
+                          static_cast<const void*>(dw_gate), static_cast<const void*>(dw_up),
+                          static_cast<const void*>(dw_down)}) {
+      if (!aligned_to(p, 2)) return invalid("tensor pointers must be aligned to their element");
+    }
+    if (rows > 0 && (!aligned_to(saved, 256) || saved_bytes < 3 * ffn_plane_bytes(b.shape))) {
+      return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");
+    }
+    if ((rc = check_workspace(workspace, workspace_bytes,
+                              ffn_backward_workspace_bytes(b.shape))) != CCV_OK) {
+      return rc;
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = begin_launches(st)) != CCV_OK) return rc;
+    return launch_ffn_backward(b, workspace, st);
+  });
+}
+
+int ccv_dropout(const void* x, int x_dtype, const void* residual, void* y, int y_dtype,
+                int64_t count, double p, uint64_t seed, uint64_t offset,
+                const int64_t* offset_device, ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    if (!valid_dtype(x_dtype) || !valid_dtype(y_dtype)) return invalid("unknown element type");
+    if (count < 0) return invalid("count must be non-negative");
+    if (count > kMaxElements) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
+    if (!(p >= 0.0 && p <= 1.0)) return invalid("p must be between 0 and 1");
+    if (residual == nullptr && y_dtype != x_dtype) {
+      return invalid("without a residual the output has the input's type");
+    }
+    if (x_dtype != CCV_DTYPE_F32 && y_dtype != CCV_DTYPE_F32 && y_dtype != x_dtype) {
+      return invalid("a 16-bit input takes a residual of its own type or float32");
+    }
+    if (count == 0) return CCV_OK;
+    if (x == nullptr || y == nullptr) return invalid("null tensor pointer");
+    if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(y, dtype_bytes(y_dtype)) ||
+        !aligned_to(residual, dtype_bytes(y_dtype)) || !aligned_to(offset_device, 8)) {
+      return invalid("tensor pointers must be aligned to their element");
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const int rc = begin_launches(st);
+    if (rc != CCV_OK) return rc;
+    Dropout a = {x, residual, y, count, x_dtype, y_dtype, p, seed, offset, offset_device};
+    return launch_dropout(a, st);
+  });
+}
+
+}  // extern "C"

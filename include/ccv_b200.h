@@ -244,6 +244,83 @@ int ccv_wgrad_planar(const float* x_real, const float* x_imag, const float* dy_r
                      const ccv_conv_shape* shape, void* workspace, size_t workspace_bytes,
                      ccv_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Token operators - no counterpart in the reference.  They work on rows of
+ * features, such as the pixels of the NHWC planes that ccv_fprop_planar
+ * writes: layer norm, a gated feed-forward block and dropout, so that a
+ * block  out = residual + dropout(ffn(layer_norm(x)))  follows a convolution
+ * in the same library.  Matrices are row-major; "row stride" is in elements
+ * and the features of a row are adjacent; outputs are dense.  Pointers are
+ * aligned to their element (16-byte aligned bases, and row lengths and
+ * strides that are multiples of 16 bytes, take the wide loads).  Zero rows
+ * are allowed.  Sums are in fp32; 16-bit results are rounded to nearest. */
+enum ccv_dtype { CCV_DTYPE_F32 = 0, CCV_DTYPE_BF16 = 1, CCV_DTYPE_F16 = 2 };
+
+/* SILU: g / (1 + exp(-g)).  GELU: g (1 + erf(g / sqrt 2)) / 2. */
+enum ccv_activation { CCV_ACTIVATION_SILU = 0, CCV_ACTIVATION_GELU = 1 };
+
+/* Layer norm of each row:
+ *   y_j = (x_j - mean) rstd weight_j + bias_j,
+ *   rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ * weight and bias (each may be null: 1 and 0) are fp32 or of x's type; y is
+ * of x's type or fp32, or any type for fp32 x.  mean and rstd (fp32, [rows])
+ * are written when not null. */
+int ccv_layer_norm_forward(const void* x, int x_dtype, int64_t x_row_stride, const void* weight,
+                           const void* bias, int weight_dtype, float eps, void* y, int y_dtype,
+                           float* mean, float* rstd, int64_t rows, int64_t features,
+                           ccv_stream_t stream);
+
+/* Gradients of ccv_layer_norm_forward from dy (of y's type) and the stored
+ * mean and rstd: dx (of x's type), dweight and dbias (of the weight's type),
+ * each skipped when null.  Deterministic.  workspace: 256-byte aligned. */
+size_t ccv_layer_norm_backward_workspace_bytes(int64_t rows, int64_t features);
+int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, const void* x,
+                            int x_dtype, int64_t x_row_stride, const float* mean,
+                            const float* rstd, const void* weight, int weight_dtype, void* dx,
+                            void* dweight, void* dbias, int64_t rows, int64_t features,
+                            void* workspace, size_t workspace_bytes, ccv_stream_t stream);
+
+/* Gated feed-forward block:
+ *   y = (act(x w_gate^T) * (x w_up^T)) w_down^T
+ * x [rows][features], w_gate and w_up [hidden][features] dense, w_down
+ * [features][hidden] dense, y [rows][features]; all bf16 or all fp16.
+ * saved (null for inference): ccv_gated_ffn_saved_bytes(), 256-byte aligned,
+ * filled with what the backward pass reads (an opaque layout).  The
+ * intermediate rows are rounded to 16 bits once each, as operands of the
+ * next product. */
+size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden);
+size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden);
+int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gate,
+                          const void* w_up, const void* w_down, void* y, int dtype,
+                          int activation, int64_t rows, int64_t features, int64_t hidden,
+                          void* saved, size_t saved_bytes, void* workspace,
+                          size_t workspace_bytes, ccv_stream_t stream);
+
+/* Gradients of ccv_gated_ffn_forward: dx [rows][features], dw_gate and dw_up
+ * [hidden][features], dw_down [features][hidden], each skipped when null.
+ * saved is what the forward call filled.  Deterministic. */
+size_t ccv_gated_ffn_backward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden);
+int ccv_gated_ffn_backward(const void* dy, int64_t dy_row_stride, const void* x,
+                           int64_t x_row_stride, const void* w_gate, const void* w_up,
+                           const void* w_down, const void* saved, size_t saved_bytes, void* dx,
+                           void* dw_gate, void* dw_up, void* dw_down, int dtype, int activation,
+                           int64_t rows, int64_t features, int64_t hidden, void* workspace,
+                           size_t workspace_bytes, ccv_stream_t stream);
+
+/* Dropout of `count` adjacent elements, with residual added when not null:
+ *   y_i = (part_i >= t ? x_i * 65536 / (65536 - t) : 0) + residual_i,
+ *   t = floor(65536 p + 1/2)
+ * part_i: 16 bits of Philox4x32-10 with key `seed` at counter (i / 8,
+ * offset), eight parts per counter, low half of each word first.  The same
+ * call on a gradient is the backward pass; no mask is stored.  y and
+ * residual are of x's type, or with a residual fp32 (any type for fp32 x).
+ * offset_device (null: none): an int64 on the device that replaces offset,
+ * read when the kernel runs, so that a captured graph draws a new mask each
+ * time its owner changes it. */
+int ccv_dropout(const void* x, int x_dtype, const void* residual, void* y, int y_dtype,
+                int64_t count, double p, uint64_t seed, uint64_t offset,
+                const int64_t* offset_device, ccv_stream_t stream);
+
 /* Device status word of the current device: nonzero after an in-kernel
  * bounded wait ran out (a CCV_ERR_* code).  While it is set, fprop kernels
  * on that device exit without work.  The kernel that gives up also writes a
