@@ -177,6 +177,23 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_backward(
   return {dx, dw, db};
 }
 
+// Rows that TMA can read in place where their length allows it at all.
+Rows as_tma_rows(const torch::Tensor& t) {
+  Rows r = as_rows(t);
+  const bool overlap = r.rows > 1 && r.stride < r.features;  // expanded rows
+  if (overlap || (r.features % 8 == 0 && (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 != 0 ||
+                                          (r.rows > 1 && r.stride % 8 != 0)))) {
+    r.t = t.clone(at::MemoryFormat::Contiguous);
+    r.stride = r.features;
+  }
+  if (r.rows <= 1) r.stride = r.features;
+  return r;
+}
+
+torch::Tensor aligned_weight(const torch::Tensor& w) {
+  return as_tma_rows(w.contiguous()).t;
+}
+
 struct FfnWeights {
   torch::Tensor gate, up, down;
   int64_t hidden = 0;
@@ -201,7 +218,7 @@ FfnWeights check_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
     check_like(*w, x, "weights");
     TORCH_CHECK_TYPE(w->scalar_type() == x.scalar_type(), "weights must be of the input's type");
   }
-  return {w_gate.contiguous(), w_up.contiguous(), w_down.contiguous(), f};
+  return {aligned_weight(w_gate), aligned_weight(w_up), aligned_weight(w_down), f};
 }
 
 // Columns of a plane of the saved buffer (rows of whole 16-byte units).
@@ -219,9 +236,10 @@ std::tuple<torch::Tensor, torch::Tensor> gated_ffn_forward(torch::Tensor x, torc
                                                            const std::string& activation,
                                                            bool save) {
   const int act = activation_code(activation);
-  const FfnWeights w = check_ffn(x, w_gate, w_up, w_down);
+  check_cuda(x, "x");
   c10::cuda::CUDAGuard guard(x.device());
-  const Rows r = as_rows(x);
+  const FfnWeights w = check_ffn(x, w_gate, w_up, w_down);
+  const Rows r = as_tma_rows(x);
   auto y = torch::empty(x.sizes(), x.options());
   torch::Tensor saved;
   size_t saved_bytes = 0;
@@ -229,7 +247,7 @@ std::tuple<torch::Tensor, torch::Tensor> gated_ffn_forward(torch::Tensor x, torc
     saved_bytes = ccv_gated_ffn_saved_bytes(r.rows, r.features, w.hidden);
     saved = torch::empty({3, r.rows, saved_width(w.hidden)}, x.options());
   }
-  const size_t bytes = ccv_gated_ffn_forward_workspace_bytes(r.rows, r.features, w.hidden);
+  const size_t bytes = ccv_gated_ffn_forward_workspace_bytes(r.rows, r.features, w.hidden, save);
   auto ws = scratch(bytes, x);
   check_rc(ccv_gated_ffn_forward(r.t.data_ptr(), r.stride, w.gate.data_ptr(), w.up.data_ptr(),
                                  w.down.data_ptr(), y.data_ptr(),
@@ -246,13 +264,14 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn
     torch::Tensor w_up, torch::Tensor w_down, const std::string& activation, bool need_dx,
     bool need_dgate, bool need_dup, bool need_ddown) {
   const int act = activation_code(activation);
+  check_cuda(x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
   const FfnWeights w = check_ffn(x, w_gate, w_up, w_down);
   check_like(dy, x, "dy");
   TORCH_CHECK_VALUE(dy.sizes() == x.sizes(), "dy must have the input's shape");
   TORCH_CHECK_TYPE(dy.scalar_type() == x.scalar_type(), "dy must be of the input's type");
   check_like(saved, x, "saved");
-  c10::cuda::CUDAGuard guard(x.device());
-  const Rows rx = as_rows(x), rdy = as_rows(dy);
+  const Rows rx = as_tma_rows(x), rdy = as_tma_rows(dy);
   TORCH_CHECK_VALUE(saved.scalar_type() == x.scalar_type() && saved.is_contiguous() &&
                         saved.dim() == 3 && saved.size(0) == 3 && saved.size(1) == rx.rows &&
                         saved.size(2) == saved_width(w.hidden),

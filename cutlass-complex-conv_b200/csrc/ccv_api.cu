@@ -330,6 +330,15 @@ int encode_tiled(CUtensorMap* map, const void* base, int rank, const uint64_t* d
 int encode_tiled_ex(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                     const uint64_t* strides_bytes, const uint32_t* box,
                     const uint32_t* elem_strides, TmaSwizzle swizzle, bool elem8) {
+  // 8-byte elements (complex64 moved as opaque 64-bit words) or fp32.
+  return encode_tiled_typed(
+      map, elem8 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank,
+      dims, strides_bytes, box, elem_strides, swizzle);
+}
+
+int encode_tiled_typed(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank,
+                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                       const uint32_t* elem_strides, TmaSwizzle swizzle) {
   std::call_once(g_encode_once, []() {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -354,10 +363,8 @@ int encode_tiled_ex(CUtensorMap* map, const void* base, int rank, const uint64_t
   const CUtensorMapSwizzle sw = swizzle == kSwizzle128   ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : swizzle == kSwizzleNone ? CU_TENSOR_MAP_SWIZZLE_NONE
                                                           : CU_TENSOR_MAP_SWIZZLE_64B;
-  // 8-byte elements (complex64 moved as opaque 64-bit words) or fp32.
   const CUresult r = g_encode_tiled(
-      map, elem8 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, rank,
-      const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+      map, type, rank, const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return set_error(CCV_ERR_UNSUPPORTED,

@@ -6,6 +6,18 @@
 // with x [M, D], Wg and Wu [F, D], Wd [D, F].  g, u, h, dg and du are rounded
 // to the operands' type once each: they are operands of the next product,
 // whose inputs the tensor cores take in 16 bits.
+//
+// Forward: GATE, PLAIN.  Backward: GRAD, PLAIN over two segments (dx), PLAIN
+// over three problems in one launch (the weight gradients).  This file plans
+// the tiles, builds the tensor maps and launches ccv_ffn_gemm.cuh's kernel.
+//
+// TMA wants row lengths that are multiples of 16 bytes: where D or F is not
+// a multiple of 8, the matrices with such rows are copied to padded rows in
+// the workspace first, and results come back through one.
+#include <algorithm>
+#include <mutex>
+
+#include "ccv_ffn_gemm.cuh"
 #include "ccv_internal.h"
 #include "ccv_ptx.cuh"
 #include "ccv_tokens.cuh"
@@ -14,127 +26,358 @@ namespace ccv {
 
 namespace {
 
-__device__ __forceinline__ float act_value(int act, float g) {
-  if (act == CCV_ACTIVATION_SILU) return g / (1.f + expf(-g));
-  return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-}
-
-// act(g) and act'(g).
-__device__ __forceinline__ float act_slope(int act, float g, float& value) {
-  if (act == CCV_ACTIVATION_SILU) {
-    const float s = 1.f / (1.f + expf(-g));
-    value = g * s;
-    return s * (1.f + g * (1.f - s));
-  }
-  const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-  value = g * c;
-  return c + g * 0.39894228040143268f * expf(-0.5f * g * g);
-}
-
-// Element (i, k) of an operand at base[i * si + k * sk].
-struct Operand {
-  const void* base = nullptr;
-  int64_t si = 0, sk = 0;
-};
-
-enum Mode { kPlain, kGate, kGrad };
-
-struct GemmArgs {
-  Operand a[2], b[2];  // kPlain: sum over both pairs (second optional); kGate: b[0] gate, b[1] up
-  int64_t m = 0, n = 0, k = 0;
-  void* out[3] = {};   // kPlain: C; kGate: h, g, u (g, u optional); kGrad: dg, du
-  const void* in[2] = {};  // kGrad: g, u
-  int64_t ldo = 0, ldi = 0;
-  int act = 0;
-};
-
-constexpr int kT = 64, kTk = 16;
-
-// 64 x 64 output tile per block, 4 x 4 per thread, fp32 multiply-adds.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) ffn_gemm_simple(const GemmArgs p) {
-  ptx::griddep_wait();
-  ptx::griddep_launch_dependents();
-  __shared__ float sa[kTk][kT + 1], sb[2][kTk][kT + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * kT;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kT;
-  float acc[2][4][4] = {};
-  const int pairs = MODE == kPlain && p.a[1].base != nullptr ? 2 : 1;
-  for (int pr = 0; pr < pairs; ++pr) {
-    const T* a = static_cast<const T*>(p.a[pr].base);
-    for (int64_t k0 = 0; k0 < p.k; k0 += kTk) {
-      for (int e = threadIdx.x; e < kT * kTk; e += 256) {
-        const int i = p.a[pr].sk == 1 ? e / kTk : e % kT;
-        const int k = p.a[pr].sk == 1 ? e % kTk : e / kT;
-        const bool in = m0 + i < p.m && k0 + k < p.k;
-        sa[k][i] = in ? to_f32(a[(m0 + i) * p.a[pr].si + (k0 + k) * p.a[pr].sk]) : 0.f;
-      }
-      for (int q = 0; q < (MODE == kGate ? 2 : 1); ++q) {
-        const Operand& ob = MODE == kGate ? p.b[q] : p.b[pr];
-        const T* b = static_cast<const T*>(ob.base);
-        for (int e = threadIdx.x; e < kT * kTk; e += 256) {
-          const int i = ob.sk == 1 ? e / kTk : e % kT;
-          const int k = ob.sk == 1 ? e % kTk : e / kT;
-          const bool in = n0 + i < p.n && k0 + k < p.k;
-          sb[q][k][i] = in ? to_f32(b[(n0 + i) * ob.si + (k0 + k) * ob.sk]) : 0.f;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kTk; ++k) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[0][i][j] += sa[k][ty * 4 + i] * sb[0][k][tx + 16 * j];
-            if (MODE == kGate) acc[1][i][j] += sa[k][ty * 4 + i] * sb[1][k][tx + 16 * j];
-          }
-        }
-      }
-      __syncthreads();
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-      if (m >= p.m || n >= p.n) continue;
-      const int64_t o = m * p.ldo + n;
-      if (MODE == kPlain) {
-        static_cast<T*>(p.out[0])[o] = from_f32<T>(acc[0][i][j]);
-      } else if (MODE == kGate) {
-        const float g = acc[0][i][j], u = acc[1][i][j];
-        static_cast<T*>(p.out[0])[o] = from_f32<T>(act_value(p.act, g) * u);
-        if (p.out[1] != nullptr) {
-          static_cast<T*>(p.out[1])[o] = from_f32<T>(g);
-          static_cast<T*>(p.out[2])[o] = from_f32<T>(u);
-        }
-      } else {
-        const float g = to_f32(static_cast<const T*>(p.in[0])[m * p.ldi + n]);
-        const float u = to_f32(static_cast<const T*>(p.in[1])[m * p.ldi + n]);
-        float value;
-        const float slope = act_slope(p.act, g, value);
-        static_cast<T*>(p.out[0])[o] = from_f32<T>(acc[0][i][j] * u * slope);
-        static_cast<T*>(p.out[1])[o] = from_f32<T>(acc[0][i][j] * value);
-      }
-    }
-  }
-}
-
-template <int MODE>
-int launch_gemm(const GemmArgs& a, int dtype, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((a.n + kT - 1) / kT),
-                  static_cast<unsigned>((a.m + kT - 1) / kT));
-  return launched(
-      dtype == CCV_DTYPE_BF16
-          ? launch_kernel(ffn_gemm_simple<__nv_bfloat16, MODE>, grid, dim3(256), 0, stream, 1, a)
-          : launch_kernel(ffn_gemm_simple<__half, MODE>, grid, dim3(256), 0, stream, 1, a),
-      "gated feed-forward product");
-}
+using ffn::GemmParams;
 
 int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+
+size_t align256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
+
+// Carves a workspace; with a null base it only adds up the size.
+struct Carver {
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base != nullptr ? base + used : nullptr;
+    used += align256(bytes);
+    return p;
+  }
+};
+
+// ------------------------------------------------------------ small kernels
+// Rows of 16-bit elements from one pitch to another.
+__global__ void ffn_copy_rows(const uint16_t* __restrict__ src, int64_t src_pitch,
+                              uint16_t* __restrict__ dst, int64_t dst_pitch, int64_t rows,
+                              int cols) {
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      dst[r * dst_pitch + c] = src[r * src_pitch + c];
+    }
+  }
+}
+
+int copy_rows(const void* src, int64_t src_pitch, void* dst, int64_t dst_pitch, int64_t rows,
+              int64_t cols, cudaStream_t stream) {
+  if (rows == 0) return CCV_OK;
+  return launched(launch_kernel(ffn_copy_rows,
+                                dim3(static_cast<unsigned>(std::min<int64_t>(rows, 148 * 16))),
+                                dim3(128), 0, stream, 1, static_cast<const uint16_t*>(src),
+                                src_pitch, static_cast<uint16_t*>(dst), dst_pitch, rows,
+                                static_cast<int>(cols)),
+                  "row copy");
+}
+
+struct SplitSum {
+  const float* partial;  // [splits][m][np]
+  void* out;
+  int64_t m, n, np, ldo;
+};
+struct SplitSums {
+  SplitSum s[ffn::kMaxProblems];
+  int splits;
+};
+
+// out = sum over the splits, in split order; four columns per thread.
+template <typename T>
+__global__ void ffn_split_sum(const SplitSums p) {
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const SplitSum& s = p.s[blockIdx.y];
+  const int64_t quads = s.np / 4;
+  const int64_t total = s.m * quads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t m = i / quads, c = (i - m * quads) * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.splits; ++k) {
+      const float4 v =
+          *reinterpret_cast<const float4*>(s.partial + (k * s.m + m) * s.np + c);
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
+    }
+    T* o = static_cast<T*>(s.out) + m * s.ldo + c;
+    const float f[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c + j < s.n) o[j] = from_f32<T>(f[j]);
+    }
+  }
+}
+
+// ------------------------------------------------------------ planning
+struct Extent {
+  int64_t m, n;
+};
+
+struct Plan {
+  int bn = 256;
+  int splits = 1;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t tile_count(const Extent* e, int problems, int width) {
+  int64_t t = 0;
+  for (int i = 0; i < problems; ++i) t += ceil_div(e[i].m, 256) * ceil_div(e[i].n, width);
+  return t;
+}
+
+// Tile width and reduction split by an estimate in clocks: a K step of a
+// 256 x BN tile is 2 BN clocks of multiplication at full rate, the narrower
+// tile loses some of it to its larger share of loads; a unit has a fixed
+// start and end; a split writes and sums partial results.
+Plan make_plan(const Extent* e, int problems, int64_t ksteps, bool may_split, bool gate) {
+  const int64_t clusters = std::max(1, device_sm_count() / 2);
+  Plan best;
+  double best_cost = 1e30;
+  for (int bn : {256, 128}) {
+    const int64_t tiles = tile_count(e, problems, gate ? bn / 2 : bn);
+    const double step = bn == 256 ? 512.0 : 290.0;
+    for (int splits = 1; splits <= (may_split ? 64 : 1) && splits <= ksteps; ++splits) {
+      const double waves = static_cast<double>(ceil_div(tiles * splits, clusters));
+      double cost = waves * (static_cast<double>(ceil_div(ksteps, splits)) * step + 600.0);
+      if (splits > 1) {
+        double bytes = 0;
+        for (int i = 0; i < problems; ++i) bytes += 8.0 * e[i].m * e[i].n * splits;
+        cost += 4000.0 + bytes / 3500.0;
+      }
+      if (cost < best_cost * 0.999) {
+        best_cost = cost;
+        best.bn = bn;
+        best.splits = splits;
+      }
+    }
+  }
+  return best;
+}
+
+// ------------------------------------------------------------ tensor maps
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == CCV_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+int encode_2d(CUtensorMap* map, int dtype, const void* base, int64_t inner, int64_t outer,
+              int64_t ld, int box_inner, int box_outer) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(outer)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld) * 2};
+  const uint32_t box[2] = {static_cast<uint32_t>(box_inner), static_cast<uint32_t>(box_outer)};
+  const uint32_t es[2] = {1, 1};
+  return encode_tiled_typed(map, map_type(dtype), base, 2, dims, strides, box, es,
+                            box_inner == 32 ? kSwizzle64 : kSwizzle128);
+}
+
+// A matrix in memory: `inner` adjacent elements per row, rows `ld` apart.
+struct Matrix {
+  const void* base = nullptr;
+  int64_t inner = 0, outer = 0, ld = 0;
+};
+
+template <typename T, int MODE, int BN, bool A_MN, bool B_MN>
+int launch_variant(const GemmParams& prm, cudaStream_t stream) {
+  using C = ffn::Config<MODE, BN>;
+  auto kern = ffn::ffn_gemm_kernel<T, MODE, BN, A_MN, B_MN>;
+  static std::once_flag once[64];
+  static int max_clusters[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t err = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() {
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (err != cudaSuccess) return;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * 148, 1, 1);
+    cfg.blockDim = dim3(ffn::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) {
+      max_clusters[dev & 63] = n;
+    } else {
+      cudaGetLastError();
+      max_clusters[dev & 63] = device_sm_count() / 2;
+    }
+  });
+  if (err != cudaSuccess) return cuda_error(err, "cudaFuncSetAttribute(ffn)");
+  const int clusters = std::min(prm.units, std::max(1, max_clusters[dev & 63]));
+  return launched(launch_kernel(kern, dim3(2 * clusters), dim3(ffn::kThreads), C::kSmem, stream, 0,
+                                prm),
+                  "gated feed-forward product");
+}
+
+template <int MODE, bool A_MN, bool B_MN>
+int launch_product(const GemmParams& prm, int dtype, int bn, cudaStream_t stream) {
+  if (dtype == CCV_DTYPE_BF16) {
+    return bn == 256 ? launch_variant<__nv_bfloat16, MODE, 256, A_MN, B_MN>(prm, stream)
+                     : launch_variant<__nv_bfloat16, MODE, 128, A_MN, B_MN>(prm, stream);
+  }
+  return bn == 256 ? launch_variant<__half, MODE, 256, A_MN, B_MN>(prm, stream)
+                   : launch_variant<__half, MODE, 128, A_MN, B_MN>(prm, stream);
+}
+
+// One launch under construction.
+template <int MODE, bool A_MN, bool B_MN>
+struct Product {
+  GemmParams prm = {};
+  Plan plan;
+  int dtype;
+  int64_t units = 0;
+  int rc = CCV_OK;
+
+  Product(int dtype_, const Plan& plan_, int64_t k, int act) : plan(plan_), dtype(dtype_) {
+    prm.status = device_status_ptr();
+    prm.problems = 1;
+    prm.segments = 1;
+    prm.ksteps = static_cast<int>(ceil_div(k, ffn::kStepK));
+    prm.splits = plan.splits;
+    prm.act = act;
+  }
+  void operand_a(int i, const Matrix& x) {
+    if (rc == CCV_OK) {
+      rc = encode_2d(&prm.a[i], dtype, x.base, x.inner, x.outer, x.ld, 64, A_MN ? 64 : ffn::kRows);
+    }
+  }
+  void operand_b(int i, const Matrix& x) {
+    if (rc == CCV_OK) {
+      rc = encode_2d(&prm.b[i], dtype, x.base, x.inner, x.outer, x.ld, 64,
+                     B_MN ? 64 : plan.bn / 2);
+    }
+  }
+  void result(int i, void* base, int64_t m, int64_t n, int64_t ld) {
+    if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, MODE == ffn::GATE ? 32 : 64, 32);
+  }
+  void partials(int i, void* base, int64_t m, int64_t n) {
+    const uint64_t np = static_cast<uint64_t>((n + 3) / 4 * 4);
+    const uint64_t dims[3] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m),
+                              static_cast<uint64_t>(plan.splits)};
+    const uint64_t strides[2] = {np * 4, np * 4 * static_cast<uint64_t>(m)};
+    const uint32_t box[3] = {32, 32, 1};
+    const uint32_t es[3] = {1, 1, 1};
+    if (rc == CCV_OK) {
+      rc = encode_tiled_typed(&prm.out[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, 3, dims, strides,
+                              box, es, kSwizzle128);
+    }
+  }
+  void problem(int i, int64_t m, int64_t n) {
+    ffn::Tiles& t = prm.tiles[i];
+    t.m = static_cast<int>(m);
+    t.n = static_cast<int>(n);
+    t.tiles_m = static_cast<int>(ceil_div(m, 256));
+    t.tiles_n = static_cast<int>(ceil_div(n, MODE == ffn::GATE ? plan.bn / 2 : plan.bn));
+    t.first = static_cast<int>(units);
+    units += static_cast<int64_t>(t.tiles_m) * t.tiles_n * plan.splits;
+    prm.problems = i + 1;
+  }
+  int launch(cudaStream_t stream) {
+    if (rc != CCV_OK) return rc;
+    if (prm.status == nullptr) return CCV_ERR_DEVICE;
+    if (units > 0x7fffffff) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
+    prm.units = static_cast<int>(units);
+    return launch_product<MODE, A_MN, B_MN>(prm, dtype, plan.bn, stream);
+  }
+};
+
+size_t partial_bytes(const Plan& p, const Extent& e) {
+  return p.splits > 1 ? static_cast<size_t>(p.splits) * e.m * ((e.n + 3) / 4 * 4) * 4 : 0;
+}
+
+int split_sum(const SplitSums& sums, int problems, int dtype, cudaStream_t stream) {
+  int64_t most = 0;
+  for (int i = 0; i < problems; ++i) most = std::max(most, sums.s[i].m * (sums.s[i].np / 4));
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(most, 256), 148 * 8));
+  const dim3 grid(blocks, problems);
+  return launched(dtype == CCV_DTYPE_BF16
+                      ? launch_kernel(ffn_split_sum<__nv_bfloat16>, grid, dim3(256), 0, stream, 1, sums)
+                      : launch_kernel(ffn_split_sum<__half>, grid, dim3(256), 0, stream, 1, sums),
+                  "gated feed-forward split sum");
+}
+
+// A [rows][cols] operand with rows TMA can read: itself, or its padded copy.
+struct Padded {
+  const void* src;
+  int64_t src_ld, rows, cols;
+  void* copy = nullptr;  // null: src is used
+  Matrix matrix() const {
+    return {copy != nullptr ? copy : src, cols, rows, copy != nullptr ? padded(cols) : src_ld};
+  }
+  int fill(cudaStream_t stream) const {
+    return copy != nullptr ? copy_rows(src, src_ld, copy, padded(cols), rows, cols, stream) : CCV_OK;
+  }
+};
+
+void* take_rows(Carver& c, int64_t rows, int64_t cols) {
+  return c.take(static_cast<size_t>(rows) * padded(cols) * 2);
+}
+
+struct ForwardPlan {
+  bool pad_d, pad_f;
+  Plan gate, down;
+  void *h = nullptr, *x = nullptr, *w_gate = nullptr, *w_up = nullptr, *w_down = nullptr,
+       *y = nullptr, *partial = nullptr;
+};
+
+ForwardPlan plan_forward(const FfnShape& s, bool save, Carver& c) {
+  ForwardPlan p;
+  p.pad_d = s.features % 8 != 0;
+  p.pad_f = s.hidden % 8 != 0;
+  const Extent eh = {s.rows, s.hidden}, ey = {s.rows, s.features};
+  p.gate = make_plan(&eh, 1, ceil_div(s.features, ffn::kStepK), false, true);
+  p.down = make_plan(&ey, 1, ceil_div(s.hidden, ffn::kStepK), true, false);
+  if (!save) p.h = take_rows(c, s.rows, s.hidden);
+  if (p.pad_d) {
+    p.x = take_rows(c, s.rows, s.features);
+    p.w_gate = take_rows(c, s.hidden, s.features);
+    p.w_up = take_rows(c, s.hidden, s.features);
+    if (p.down.splits == 1) p.y = take_rows(c, s.rows, s.features);
+  }
+  if (p.pad_f) p.w_down = take_rows(c, s.features, s.hidden);
+  if (p.down.splits > 1) p.partial = c.take(partial_bytes(p.down, ey));
+  return p;
+}
+
+struct BackwardPlan {
+  bool pad_d, pad_f;
+  Plan grad, dx, dw;
+  Extent dw_extent[3];
+  void *dg, *du, *dy = nullptr, *x = nullptr, *w_gate = nullptr, *w_up = nullptr,
+                 *w_down = nullptr, *out_dx = nullptr, *out_dw[3] = {}, *partial = nullptr;
+};
+
+BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
+  BackwardPlan p;
+  p.pad_d = s.features % 8 != 0;
+  p.pad_f = s.hidden % 8 != 0;
+  const Extent eh = {s.rows, s.hidden}, ex = {s.rows, s.features};
+  p.dw_extent[0] = p.dw_extent[1] = {s.hidden, s.features};
+  p.dw_extent[2] = {s.features, s.hidden};
+  p.grad = make_plan(&eh, 1, ceil_div(s.features, ffn::kStepK), false, false);
+  p.dx = make_plan(&ex, 1, 2 * ceil_div(s.hidden, ffn::kStepK), true, false);
+  p.dw = make_plan(p.dw_extent, 3, ceil_div(s.rows, ffn::kStepK), true, false);
+  p.dg = take_rows(c, s.rows, s.hidden);
+  p.du = take_rows(c, s.rows, s.hidden);
+  if (p.pad_d) {
+    p.dy = take_rows(c, s.rows, s.features);
+    p.x = take_rows(c, s.rows, s.features);
+    p.w_gate = take_rows(c, s.hidden, s.features);
+    p.w_up = take_rows(c, s.hidden, s.features);
+    if (p.dx.splits == 1) p.out_dx = take_rows(c, s.rows, s.features);
+  }
+  if (p.pad_f) p.w_down = take_rows(c, s.features, s.hidden);
+  size_t partial = partial_bytes(p.dx, ex), dw = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (p.dw.splits == 1) {
+      if (i < 2 ? p.pad_d : p.pad_f) {
+        p.out_dw[i] = take_rows(c, p.dw_extent[i].m, p.dw_extent[i].n);
+      }
+    } else {
+      dw += align256(partial_bytes(p.dw, p.dw_extent[i]));
+    }
+  }
+  p.partial = c.take(std::max(partial, dw));
+  return p;
+}
 
 }  // namespace
 
@@ -142,101 +385,163 @@ size_t ffn_plane_bytes(const FfnShape& s) {
   return static_cast<size_t>(s.rows) * padded(s.hidden) * 2;
 }
 
-size_t ffn_forward_workspace_bytes(const FfnShape& s) { return ffn_plane_bytes(s); }
-size_t ffn_backward_workspace_bytes(const FfnShape& s) { return 2 * ffn_plane_bytes(s); }
+size_t ffn_forward_workspace_bytes(const FfnShape& s, bool save) {
+  Carver c{nullptr};
+  plan_forward(s, save, c);
+  return c.used;
+}
+
+size_t ffn_backward_workspace_bytes(const FfnShape& s) {
+  Carver c{nullptr};
+  plan_backward(s, c);
+  return c.used;
+}
 
 int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   const FfnShape& s = f.shape;
-  if (s.rows == 0) return CCV_OK;
-  const int64_t fp = padded(s.hidden);
+  const int64_t m = s.rows, d = s.features, hid = s.hidden, fp = padded(hid);
   char* saved = static_cast<char*>(f.saved);
   const size_t plane = ffn_plane_bytes(s);
-  GemmArgs a;
-  a.a[0] = {f.x, f.x_stride, 1};
-  a.b[0] = {f.w_gate, s.features, 1};
-  a.b[1] = {f.w_up, s.features, 1};
-  a.m = s.rows;
-  a.n = s.hidden;
-  a.k = s.features;
-  a.act = s.activation;
-  a.ldo = fp;
-  a.out[0] = saved != nullptr ? saved : ws;
-  if (saved != nullptr) {
-    a.out[1] = saved + plane;
-    a.out[2] = saved + 2 * plane;
+  Carver c{static_cast<char*>(ws)};
+  const ForwardPlan p = plan_forward(s, saved != nullptr, c);
+  const Padded x{f.x, f.x_stride, m, d, p.x}, wg{f.w_gate, d, hid, d, p.w_gate},
+      wu{f.w_up, d, hid, d, p.w_up}, wd{f.w_down, hid, d, hid, p.w_down};
+  for (const Padded* q : {&x, &wg, &wu, &wd}) {
+    const int rc = q->fill(stream);
+    if (rc != CCV_OK) return rc;
   }
-  int rc = launch_gemm<kGate>(a, s.dtype, stream);
-  if (rc != CCV_OK) return rc;
-  GemmArgs d;
-  d.a[0] = {a.out[0], fp, 1};
-  d.b[0] = {f.w_down, s.hidden, 1};
-  d.m = s.rows;
-  d.n = s.features;
-  d.k = s.hidden;
-  d.out[0] = f.y;
-  d.ldo = s.features;
-  return launch_gemm<kPlain>(d, s.dtype, stream);
+  void* h = saved != nullptr ? saved : p.h;
+  {
+    Product<ffn::GATE, false, false> g(s.dtype, p.gate, d, s.activation);
+    g.operand_a(0, x.matrix());
+    g.operand_b(0, wg.matrix());
+    g.operand_b(1, wu.matrix());
+    g.result(0, h, m, hid, fp);
+    if (saved != nullptr) {
+      g.result(1, saved + plane, m, hid, fp);
+      g.result(2, saved + 2 * plane, m, hid, fp);
+      g.prm.save = 1;
+    }
+    g.problem(0, m, hid);
+    const int rc = g.launch(stream);
+    if (rc != CCV_OK) return rc;
+  }
+  Product<ffn::PLAIN, false, false> y(s.dtype, p.down, hid, 0);
+  y.operand_a(0, {h, hid, m, fp});
+  y.operand_b(0, wd.matrix());
+  y.problem(0, m, d);
+  if (p.down.splits > 1) {
+    y.partials(0, p.partial, m, d);
+    const int rc = y.launch(stream);
+    if (rc != CCV_OK) return rc;
+    SplitSums sums = {};
+    sums.splits = p.down.splits;
+    sums.s[0] = {static_cast<const float*>(p.partial), f.y, m, d, (d + 3) / 4 * 4, d};
+    return split_sum(sums, 1, s.dtype, stream);
+  }
+  y.result(0, p.y != nullptr ? p.y : f.y, m, d, p.y != nullptr ? padded(d) : d);
+  const int rc = y.launch(stream);
+  if (rc != CCV_OK || p.y == nullptr) return rc;
+  return copy_rows(p.y, padded(d), f.y, d, m, d, stream);
 }
 
 int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
   const FfnShape& s = b.shape;
-  const int64_t fp = padded(s.hidden);
+  const int64_t m = s.rows, d = s.features, hid = s.hidden, fp = padded(hid);
   const size_t plane = ffn_plane_bytes(s);
   const char* saved = static_cast<const char*>(b.saved);
-  char* dg = static_cast<char*>(ws);
-  char* du = dg + plane;
-  int rc = CCV_OK;
-  if (s.rows > 0 && (b.dx != nullptr || b.dw_gate != nullptr || b.dw_up != nullptr)) {
-    GemmArgs a;
-    a.a[0] = {b.dy, b.dy_stride, 1};
-    a.b[0] = {b.w_down, 1, s.hidden};
-    a.m = s.rows;
-    a.n = s.hidden;
-    a.k = s.features;
-    a.in[0] = saved + plane;
-    a.in[1] = saved + 2 * plane;
-    a.ldi = fp;
-    a.out[0] = dg;
-    a.out[1] = du;
-    a.ldo = fp;
-    a.act = s.activation;
-    if ((rc = launch_gemm<kGrad>(a, s.dtype, stream)) != CCV_OK) return rc;
+  void* const dw[3] = {b.dw_gate, b.dw_up, b.dw_down};
+  if (m == 0) {
+    for (void* w : dw) {
+      if (w == nullptr) continue;
+      const int rc = launched(cudaMemsetAsync(w, 0, static_cast<size_t>(d) * hid * 2, stream),
+                              "cudaMemsetAsync");
+      if (rc != CCV_OK) return rc;
+    }
+    return CCV_OK;
   }
-  if (s.rows > 0 && b.dx != nullptr) {
-    GemmArgs a;
-    a.a[0] = {dg, fp, 1};
-    a.a[1] = {du, fp, 1};
-    a.b[0] = {b.w_gate, 1, s.features};
-    a.b[1] = {b.w_up, 1, s.features};
-    a.m = s.rows;
-    a.n = s.features;
-    a.k = s.hidden;
-    a.out[0] = b.dx;
-    a.ldo = s.features;
-    if ((rc = launch_gemm<kPlain>(a, s.dtype, stream)) != CCV_OK) return rc;
+  Carver c{static_cast<char*>(ws)};
+  const BackwardPlan p = plan_backward(s, c);
+  const bool need_grad = b.dx != nullptr || dw[0] != nullptr || dw[1] != nullptr;
+  const Padded dy{b.dy, b.dy_stride, m, d, p.dy}, x{b.x, b.x_stride, m, d, p.x},
+      wg{b.w_gate, d, hid, d, p.w_gate}, wu{b.w_up, d, hid, d, p.w_up},
+      wd{b.w_down, hid, d, hid, p.w_down};
+  int rc = dy.fill(stream);
+  if (rc == CCV_OK && (dw[0] != nullptr || dw[1] != nullptr)) rc = x.fill(stream);
+  if (rc == CCV_OK && need_grad) rc = wd.fill(stream);
+  if (rc == CCV_OK && b.dx != nullptr) rc = wg.fill(stream);
+  if (rc == CCV_OK && b.dx != nullptr) rc = wu.fill(stream);
+  if (rc != CCV_OK) return rc;
+  if (need_grad) {
+    Product<ffn::GRAD, false, true> g(s.dtype, p.grad, d, s.activation);
+    g.operand_a(0, dy.matrix());
+    g.operand_b(0, wd.matrix());
+    g.result(0, p.dg, m, hid, fp);
+    g.result(1, p.du, m, hid, fp);
+    for (int i = 0; i < 2 && g.rc == CCV_OK; ++i) {
+      g.rc = encode_2d(&g.prm.in[i], s.dtype, saved + (i + 1) * plane, hid, m, fp, 64, 32);
+    }
+    g.problem(0, m, hid);
+    if ((rc = g.launch(stream)) != CCV_OK) return rc;
   }
-  const struct {
-    void* out;
-    Operand a, b;
-    int64_t m, n;
-  } grads[3] = {
-      {b.dw_gate, {dg, 1, fp}, {b.x, 1, b.x_stride}, s.hidden, s.features},
-      {b.dw_up, {du, 1, fp}, {b.x, 1, b.x_stride}, s.hidden, s.features},
-      {b.dw_down, {b.dy, 1, b.dy_stride}, {saved, 1, fp}, s.features, s.hidden},
-  };
-  for (const auto& g : grads) {
-    if (g.out == nullptr) continue;
-    GemmArgs a;
-    a.a[0] = g.a;
-    a.b[0] = g.b;
-    a.m = g.m;
-    a.n = g.n;
-    a.k = s.rows;
-    a.out[0] = g.out;
-    a.ldo = g.n;
-    if ((rc = launch_gemm<kPlain>(a, s.dtype, stream)) != CCV_OK) return rc;
+  if (b.dx != nullptr) {
+    Product<ffn::PLAIN, false, true> g(s.dtype, p.dx, hid, 0);
+    g.prm.segments = 2;
+    g.operand_a(0, {p.dg, hid, m, fp});
+    g.operand_a(1, {p.du, hid, m, fp});
+    g.operand_b(0, wg.matrix());
+    g.operand_b(1, wu.matrix());
+    g.problem(0, m, d);
+    if (p.dx.splits > 1) {
+      g.partials(0, p.partial, m, d);
+      if ((rc = g.launch(stream)) != CCV_OK) return rc;
+      SplitSums sums = {};
+      sums.splits = p.dx.splits;
+      sums.s[0] = {static_cast<const float*>(p.partial), b.dx, m, d, (d + 3) / 4 * 4, d};
+      if ((rc = split_sum(sums, 1, s.dtype, stream)) != CCV_OK) return rc;
+    } else {
+      void* out = p.out_dx != nullptr ? p.out_dx : b.dx;
+      g.result(0, out, m, d, p.out_dx != nullptr ? padded(d) : d);
+      if ((rc = g.launch(stream)) != CCV_OK) return rc;
+      if (p.out_dx != nullptr &&
+          (rc = copy_rows(out, padded(d), b.dx, d, m, d, stream)) != CCV_OK) {
+        return rc;
+      }
+    }
   }
-  return rc;
+  const Matrix left[3] = {{p.dg, hid, m, fp}, {p.du, hid, m, fp}, dy.matrix()};
+  const Matrix right[3] = {x.matrix(), x.matrix(), {saved, hid, m, fp}};
+  Product<ffn::PLAIN, true, true> g(s.dtype, p.dw, m, 0);
+  SplitSums sums = {};
+  sums.splits = p.dw.splits;
+  int count = 0;
+  char* partial = static_cast<char*>(p.partial);
+  for (int i = 0; i < 3; ++i) {
+    if (dw[i] == nullptr) continue;
+    const Extent& e = p.dw_extent[i];
+    g.operand_a(count, left[i]);
+    g.operand_b(count, right[i]);
+    g.problem(count, e.m, e.n);
+    if (p.dw.splits > 1) {
+      g.partials(count, partial, e.m, e.n);
+      sums.s[count] = {reinterpret_cast<const float*>(partial), dw[i], e.m, e.n, (e.n + 3) / 4 * 4,
+                       e.n};
+      partial += align256(partial_bytes(p.dw, e));
+    } else {
+      void* out = p.out_dw[i] != nullptr ? p.out_dw[i] : dw[i];
+      g.result(count, out, e.m, e.n, p.out_dw[i] != nullptr ? padded(e.n) : e.n);
+    }
+    ++count;
+  }
+  if (count == 0) return CCV_OK;
+  if ((rc = g.launch(stream)) != CCV_OK) return rc;
+  if (p.dw.splits > 1) return split_sum(sums, count, s.dtype, stream);
+  for (int i = 0; i < 3; ++i) {
+    if (dw[i] == nullptr || p.out_dw[i] == nullptr) continue;
+    const Extent& e = p.dw_extent[i];
+    if ((rc = copy_rows(p.out_dw[i], padded(e.n), dw[i], e.n, e.m, e.n, stream)) != CCV_OK) return rc;
+  }
+  return CCV_OK;
 }
 
 }  // namespace ccv

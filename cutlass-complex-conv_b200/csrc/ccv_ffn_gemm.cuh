@@ -1,0 +1,555 @@
+// Matrix products of the gated feed-forward block on tcgen05, one persistent
+// kernel template for all of them:
+//   GATE   h = act(x Wg^T) (x Wu^T)        epilogue: activation and product
+//   PLAIN  c = a b (+ a' b')               down projection, dx, weight gradients
+//   GRAD   dh = dy Wd                      epilogue: dg, du from dh, g, u
+//
+// A cluster of two CTAs computes a tile of 256 x BN with
+// tcgen05.mma.cta_group::2: each CTA holds 128 rows of A and half of B's BN
+// columns in shared memory and its 128 rows of the fp32 sums in TMEM.  Per
+// K step of 64 a CTA loads 16 KB of A and 64 BN bytes of B (TMA, 128-byte
+// swizzle).  For GATE, one CTA's half of B is the gate projection's rows and
+// the other's the up projection's, so the sums of g and u of one output lie
+// in the same TMEM lane, BN / 2 columns apart, and the epilogue needs no
+// exchange.  Operands whose reduction index is not innermost in memory (the
+// weights in dh and dx, both operands of the weight gradients) are loaded as
+// they lie and multiplied through the M/N-innermost descriptor form: nothing
+// is transposed.
+//
+// Two accumulators in TMEM let eight epilogue warps work on one tile while
+// the next is multiplied; they pass their results through swizzled
+// shared-memory slots to TMA stores, which clip the ragged edges.
+//
+// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue (even CTA), 2-9
+// epilogue (quarter of the rows = warp % 4, half of the columns).
+#pragma once
+
+#include <cuda.h>
+
+#include "ccv_internal.h"
+#include "ccv_ptx.cuh"
+#include "ccv_tokens.cuh"
+
+namespace ccv {
+namespace ffn {
+
+enum Mode { GATE, PLAIN, GRAD };
+
+constexpr int kRows = 128;        // rows of one CTA's tile
+constexpr int kStepK = 64;        // reduction elements per pipeline stage: 128-byte rows
+constexpr int kOperandA = kRows * kStepK * 2;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kSlotBytes = 8192;  // staging of one epilogue warp
+constexpr int kMaxProblems = 3;
+constexpr int kRasterRows = 8;    // tile rows walked together (operand reuse in L2)
+constexpr int kTimeoutCode = CCV_ERR_DEVICE_TIMEOUT;
+
+struct Tiles {
+  int m, n;              // extents of the result
+  int tiles_m, tiles_n;
+  int first;             // first work unit
+};
+
+struct alignas(64) GemmParams {
+  // One problem: segments of the reduction, a[s] with b[s] (GATE: b[0] gate
+  // rows, b[1] up rows).  Several problems: one segment each.
+  CUtensorMap a[kMaxProblems], b[kMaxProblems];
+  CUtensorMap out[kMaxProblems];  // GATE: h, g, u; GRAD: dg, du; PLAIN: per problem
+  CUtensorMap in[2];              // GRAD: g, u
+  Tiles tiles[kMaxProblems];
+  int* status;
+  int problems, segments;
+  int ksteps;   // per segment
+  int splits;   // PLAIN: parts of the reduction, summed by ffn_split_sum
+  int units;
+  int save;     // GATE: store g and u too
+  int act;
+};
+
+template <int MODE, int BN>
+struct Config {
+  static constexpr int kOperandB = BN / 2 * kStepK * 2;
+  static constexpr int kStage = kOperandA + kOperandB;
+  static constexpr int kStaging = kEpiWarps * kSlotBytes;
+  static constexpr int kStages = BN == 256 ? 5 : 6;
+  static constexpr int kStagingOffset = kStages * kStage;
+  static constexpr int kBarOffset = kStagingOffset + kStaging;
+  static constexpr int kBarBytes = 512;
+  static constexpr int kSmem = kBarOffset + kBarBytes + 1024;
+  static constexpr int kTmemCols = 2 * BN;
+  static_assert(kSmem <= 232448, "shared memory");
+  static_assert((2 * kStages + 5 + kEpiWarps) * 8 + 16 <= kBarBytes, "barriers");
+};
+
+struct Unit {
+  int problem, tm, tn, split, k0, k1;
+};
+
+__device__ __forceinline__ Unit decode(const GemmParams& p, int u) {
+  Unit w;
+  w.problem = 0;
+#pragma unroll
+  for (int i = 1; i < kMaxProblems; ++i) {
+    if (i < p.problems && u >= p.tiles[i].first) w.problem = i;
+  }
+  const Tiles& t = p.tiles[w.problem];
+  const int local = u - t.first;
+  const int tile = local / p.splits;
+  w.split = local - tile * p.splits;
+  // Bands of kRasterRows tile rows, walked column by column.
+  const int band = tile / (kRasterRows * t.tiles_n);
+  const int r = tile - band * kRasterRows * t.tiles_n;
+  const int rows = min(kRasterRows, t.tiles_m - band * kRasterRows);
+  w.tn = r / rows;
+  w.tm = band * kRasterRows + (r - w.tn * rows);
+  const int total = p.ksteps * p.segments;
+  w.k0 = static_cast<int>(static_cast<long long>(total) * w.split / p.splits);
+  w.k1 = static_cast<int>(static_cast<long long>(total) * (w.split + 1) / p.splits);
+  return w;
+}
+
+// act(g): the sigmoid from the hardware exponential and reciprocal.  GELU's
+// normal distribution is Abramowitz and Stegun 7.1.26 (|error of erf| <=
+// 1.5e-7), a polynomial times exp(-g^2/2), the exponential its slope needs
+// too.  Both errors lie far below the 16-bit rounding of the result.
+__device__ __forceinline__ void activation(int act, float g, float& value, float& slope) {
+  if (act == CCV_ACTIVATION_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    value = g * s;
+    slope = s * (1.f + g * (1.f - s));
+  } else {
+    const float x = fabsf(g) * 0.70710678118654752f;
+    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+    const float e = __expf(-x * x);
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f);
+    const float tail = 0.5f * t * q * e;
+    const float c = g >= 0.f ? 1.f - tail : tail;
+    value = g * c;
+    slope = fmaf(g * 0.39894228040143268f, e, c);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// 16-byte unit `j` of row `row` of a slot with 64- or 128-byte rows, where
+// TMA's swizzle of that width puts it.
+__device__ __forceinline__ uint32_t slot64(uint32_t slot, int row, int j) {
+  return slot + row * 64 + ((j ^ ((row >> 1) & 3)) << 4);
+}
+__device__ __forceinline__ uint32_t slot128(uint32_t slot, int row, int j) {
+  return slot + row * 128 + ((j ^ (row & 7)) << 4);
+}
+
+// An epilogue warp's ring of staging slots of BYTES each, written by its
+// lanes and read by TMA stores.
+template <int BYTES>
+struct Ring {
+  static constexpr int kSlots = kSlotBytes / BYTES;
+  uint32_t base;
+  uint32_t next = 0;
+  // A slot no store still reads.
+  __device__ __forceinline__ uint32_t take(int lane) {
+    if (lane == 0) ptx::bulk_wait_read_le<kSlots - 1>();
+    __syncwarp();
+    const uint32_t s = base + (next % kSlots) * BYTES;
+    ++next;
+    return s;
+  }
+};
+
+// Makes the lanes' slot writes visible to the async proxy; then lane 0 stores.
+__device__ __forceinline__ void publish() {
+  ptx::fence_proxy_async_shared();
+  __syncwarp();
+}
+
+template <typename T, int MODE, int BN, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    ffn_gemm_kernel(const __grid_constant__ GemmParams p) {
+  using C = Config<MODE, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+  // full[S] (even CTA), empty[S], tfull[2], tempty[2] (even CTA), done,
+  // loaded[8] (GRAD: an epilogue warp's g and u), the TMEM address, flags.
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 5 + kEpiWarps);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_holder + 1);  // [0] skip, [1] abort
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cid = static_cast<int>(ptx::cluster_id_x());
+  const int ncl = static_cast<int>(ptx::nclusters_x());
+  const uint32_t smem_base = ptx::smem_u32(smem);
+  const uint32_t bar_base = ptx::smem_u32(bars);
+  auto full_bar = [&](int i) { return bar_base + 8u * i; };
+  auto empty_bar = [&](int i) { return bar_base + 8u * (C::kStages + i); };
+  auto tfull_bar = [&](int b) { return bar_base + 8u * (2 * C::kStages + b); };
+  auto tempty_bar = [&](int b) { return bar_base + 8u * (2 * C::kStages + 2 + b); };
+  const uint32_t done_bar = bar_base + 8u * (2 * C::kStages + 4);
+  const uint32_t loaded_bar0 = bar_base + 8u * (2 * C::kStages + 5);
+
+  if (threadIdx.x == 0) {
+    flags[1] = 0;
+    for (int i = 0; i < C::kStages; ++i) {
+      ptx::mbar_init(full_bar(i), 1);
+      ptx::mbar_init(empty_bar(i), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(tfull_bar(b), 1);
+      ptx::mbar_init(tempty_bar(b), 2 * kEpiWarps);  // both CTAs' epilogue warps
+    }
+    ptx::mbar_init(done_bar, 1);
+    for (int i = 0; i < kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&p.a[0]);
+    ptx::prefetch_tmap(&p.b[MODE == GATE ? rank : 0]);
+    ptx::prefetch_tmap(&p.out[0]);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(tmem_holder), C::kTmemCols);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  ptx::tc_fence_after();
+  // Everything above may overlap the previous kernel on the stream.
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  if (threadIdx.x == 0) flags[0] = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
+  ptx::cta_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  const bool skip = flags[0] != 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0 && !skip) {
+      uint32_t g = 0;
+      bool abort = false;
+      for (int u = cid; u < p.units && !abort; u += ncl) {
+        const Unit w = decode(p, u);
+        const int m0 = (2 * w.tm + static_cast<int>(rank)) * kRows;
+        const int n0 = MODE == GATE ? w.tn * (BN / 2) : w.tn * BN + static_cast<int>(rank) * (BN / 2);
+        for (int ks = w.k0; ks < w.k1; ++ks, ++g) {
+          const int stage = static_cast<int>(g % C::kStages);
+          if (!ptx::mbar_wait_bounded(empty_bar(stage), ((g / C::kStages) & 1u) ^ 1u, p.status,
+                                      kTimeoutCode) ||
+              flags[1]) {
+            flags[1] = 1;
+            abort = true;
+            break;
+          }
+          if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * C::kStage);
+          const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0);
+          const int seg = ks >= p.ksteps ? 1 : 0;
+          const int k = (ks - seg * p.ksteps) * kStepK;
+          const int map = p.problems > 1 ? w.problem : seg;
+          const CUtensorMap* ma = &p.a[map];
+          const CUtensorMap* mb = &p.b[MODE == GATE ? static_cast<int>(rank) : map];
+          const uint32_t sa = smem_base + stage * C::kStage;
+          const uint32_t sb = sa + kOperandA;
+          if constexpr (A_MN) {
+            ptx::tma_load_2d_pair(sa, ma, fb, m0, k);
+            ptx::tma_load_2d_pair(sa + 8192, ma, fb, m0 + 64, k);
+          } else {
+            ptx::tma_load_2d_pair(sa, ma, fb, k, m0);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int i = 0; i < BN / 128; ++i) {
+              ptx::tma_load_2d_pair(sb + 8192 * i, mb, fb, n0 + 64 * i, k);
+            }
+          } else {
+            ptx::tma_load_2d_pair(sb, mb, fb, k, n0);
+          }
+        }
+      }
+      if (leader) {
+        // Drain: every issued stage's bytes (both CTAs) have landed.
+        for (uint32_t j = 0; j < static_cast<uint32_t>(C::kStages) && j < g; ++j) {
+          const uint32_t gg = g - 1 - j;
+          ptx::mbar_wait_bounded(full_bar(static_cast<int>(gg % C::kStages)),
+                                 (gg / C::kStages) & 1u, p.status, kTimeoutCode);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (even CTA)
+    if (leader && lane == 0 && !skip) {
+      constexpr uint32_t idesc = ptx::idesc_f16(2 * kRows, BN, kIsBf16<T>, A_MN,
+                                                B_MN);
+      uint32_t g = 0;
+      int i = 0;
+      bool abort = false;
+      for (int u = cid; u < p.units && !abort; u += ncl, ++i) {
+        const Unit w = decode(p, u);
+        const int buf = i & 1;
+        const uint32_t use = static_cast<uint32_t>(i >> 1);
+        if (!ptx::mbar_wait_bounded(tempty_bar(buf), (use & 1u) ^ 1u, p.status, kTimeoutCode)) {
+          flags[1] = 1;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(buf * BN);
+        for (int ks = w.k0; ks < w.k1; ++ks, ++g) {
+          const int stage = static_cast<int>(g % C::kStages);
+          if (!ptx::mbar_wait_bounded(full_bar(stage), (g / C::kStages) & 1u, p.status,
+                                      kTimeoutCode)) {
+            flags[1] = 1;
+            abort = true;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t sa = smem_base + stage * C::kStage;
+          const uint32_t sb = sa + kOperandA;
+#pragma unroll
+          for (int kk = 0; kk < kStepK / 16; ++kk) {
+            const uint64_t da = A_MN ? ptx::desc_mnmajor_sw128(sa + kk * 2048, 8192)
+                                     : ptx::desc_kmajor_sw128(sa + kk * 32);
+            const uint64_t db = B_MN ? ptx::desc_mnmajor_sw128(sb + kk * 2048, 8192)
+                                     : ptx::desc_kmajor_sw128(sb + kk * 32);
+            ptx::mma_f16_pair(d, da, db, idesc, (ks != w.k0 || kk != 0) ? 1u : 0u);
+          }
+          ptx::mma_commit_pair(empty_bar(stage));
+        }
+        ptx::mma_commit_pair(tfull_bar(buf));
+      }
+      // All issued MMAs complete before teardown.
+      ptx::mma_commit_pair(done_bar);
+      ptx::mbar_wait_bounded(done_bar, 0, p.status, kTimeoutCode);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int e = warp - 2;
+    const int quarter = warp & 3;
+    const int half = e >> 2;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t staging = smem_base + C::kStagingOffset + e * kSlotBytes;
+    const uint32_t loaded = loaded_bar0 + 8u * e;
+    const uint32_t tempty0 = ptx::mapa_shared(tempty_bar(0), 0);
+    const uint32_t tempty1 = ptx::mapa_shared(tempty_bar(1), 0);
+    Ring<2048> ring2{staging};
+    Ring<4096> ring4{staging};
+    uint32_t loads = 0;
+    int i = 0;
+    for (int u = cid; u < p.units && !skip; u += ncl, ++i) {
+      const Unit w = decode(p, u);
+      const Tiles& t = p.tiles[w.problem];
+      const int buf = i & 1;
+      const uint32_t use = static_cast<uint32_t>(i >> 1);
+      const int row0 = (2 * w.tm + static_cast<int>(rank)) * kRows + quarter * 32;
+      const bool rows_in = row0 < t.m;
+      const uint32_t acc = t_row + static_cast<uint32_t>(buf * BN);
+      constexpr int kGradChunks = BN / 2 / 64;
+      // GRAD: g and u of this warp's first 64 columns arrive during the mainloop.
+      auto load_inputs = [&](int col) {
+        if (lane == 0) {
+          ptx::bulk_wait_read_all();
+          ptx::mbar_arrive_expect_tx(loaded, 8192);
+          ptx::tma_load_2d(staging, &p.in[0], loaded, col, row0);
+          ptx::tma_load_2d(staging + 4096, &p.in[1], loaded, col, row0);
+        }
+      };
+      const int grad_col = w.tn * BN + half * (BN / 2);
+      if constexpr (MODE == GRAD) load_inputs(grad_col);
+      bool ok = ptx::mbar_wait_bounded_backoff(tfull_bar(buf), use & 1u, p.status, kTimeoutCode);
+      ptx::tc_fence_after();
+      if (!ok) flags[1] = 1;
+      const bool store = ok && !flags[1];
+      if constexpr (MODE == GATE) {
+        // BN / 4 outputs per warp, 32 at a time.
+#pragma unroll 1
+        for (int c = 0; c < BN / 4; c += 32) {
+          const int fc = half * (BN / 4) + c;
+          uint32_t g[32], v[32];
+          ptx::tmem_ld_32x32b_x32(acc + fc, g);
+          ptx::tmem_ld_32x32b_x32(acc + BN / 2 + fc, v);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(g);
+          ptx::reg_fence(v);
+          const int col = w.tn * (BN / 2) + fc;
+          const bool in = store && rows_in && col < t.n;
+          auto put = [&](auto&& value, const CUtensorMap* map) {
+            const uint32_t slot = ring2.take(lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t q[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                q[k] = pack2(value(8 * j + 2 * k), value(8 * j + 2 * k + 1), T());
+              }
+              st_shared_v4(slot64(slot, lane, j), q[0], q[1], q[2], q[3]);
+            }
+            publish();
+            if (lane == 0) {
+              if (in) ptx::tma_store_2d(map, slot, col, row0);
+              ptx::bulk_commit_group();
+            }
+          };
+          put([&](int j) {
+            float value, slope;
+            activation(p.act, __uint_as_float(g[j]), value, slope);
+            return value * __uint_as_float(v[j]);
+          }, &p.out[0]);
+          if (p.save) {
+            put([&](int j) { return __uint_as_float(g[j]); }, &p.out[1]);
+            put([&](int j) { return __uint_as_float(v[j]); }, &p.out[2]);
+          }
+        }
+      } else if constexpr (MODE == GRAD) {
+#pragma unroll 1
+        for (int c = 0; c < kGradChunks; ++c) {
+          const int col = grad_col + c * 64;
+          ok = ptx::mbar_wait_bounded_backoff(loaded, loads & 1u, p.status, kTimeoutCode) && ok;
+          ++loads;
+          if (!ok) flags[1] = 1;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t d[32];
+            ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 64 + h * 32, d);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence(d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t ag = slot128(staging, lane, h * 4 + j);
+              const uint32_t au = slot128(staging + 4096, lane, h * 4 + j);
+              const uint4 g4 = ld_shared_v4(ag), u4 = ld_shared_v4(au);
+              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+              uint32_t og[4], ou[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 gg = unpack2(gw[k], T()), uu = unpack2(uw[k], T());
+                const float d0 = __uint_as_float(d[8 * j + 2 * k]);
+                const float d1 = __uint_as_float(d[8 * j + 2 * k + 1]);
+                float v0, s0, v1, s1;
+                activation(p.act, gg.x, v0, s0);
+                activation(p.act, gg.y, v1, s1);
+                og[k] = pack2(d0 * uu.x * s0, d1 * uu.y * s1, T());
+                ou[k] = pack2(d0 * v0, d1 * v1, T());
+              }
+              // The results take the place of the inputs they came from.
+              st_shared_v4(ag, og[0], og[1], og[2], og[3]);
+              st_shared_v4(au, ou[0], ou[1], ou[2], ou[3]);
+            }
+          }
+          publish();
+          if (lane == 0) {
+            if (ok && !flags[1] && rows_in && col < t.n) {
+              ptx::tma_store_2d(&p.out[0], staging, col, row0);
+              ptx::tma_store_2d(&p.out[1], staging + 4096, col, row0);
+            }
+            ptx::bulk_commit_group();
+          }
+          if (c + 1 < kGradChunks) load_inputs(col + 64);
+        }
+      } else if (p.splits > 1) {
+        // fp32 partial sums, 32 columns at a time: [problem][split][m][n].
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 32) {
+          uint32_t d[32];
+          ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c, d);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(d);
+          const int col = w.tn * BN + half * (BN / 2) + c;
+          const uint32_t slot = ring4.take(lane);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            st_shared_v4(slot128(slot, lane, j), d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
+          }
+          publish();
+          if (lane == 0) {
+            if (store && rows_in && col < t.n) {
+              ptx::tma_store_3d(&p.out[w.problem], slot, col, row0, w.split);
+            }
+            ptx::bulk_commit_group();
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 64) {
+          const int col = w.tn * BN + half * (BN / 2) + c;
+          const uint32_t slot = ring4.take(lane);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t d[32];
+            ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c + h * 32, d);
+            ptx::tmem_wait_ld();
+            ptx::reg_fence(d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t q[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                q[k] = pack2(__uint_as_float(d[8 * j + 2 * k]),
+                             __uint_as_float(d[8 * j + 2 * k + 1]), T());
+              }
+              st_shared_v4(slot128(slot, lane, h * 4 + j), q[0], q[1], q[2], q[3]);
+            }
+          }
+          publish();
+          if (lane == 0) {
+            if (store && rows_in && col < t.n) ptx::tma_store_2d(&p.out[w.problem], slot, col, row0);
+            ptx::bulk_commit_group();
+          }
+        }
+      }
+      // This warp is done with the accumulator: release it to the MMA issuer.
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(buf == 0 ? tempty0 : tempty1);
+      if (!ok) break;
+    }
+    // Output stores still in flight complete before the CTA exits.
+    if (lane == 0) ptx::bulk_wait_all();
+  }
+
+  ptx::cta_sync();
+  if (flags[1]) ptx::nanosleep(100000);  // let stray copies of an aborted tile land
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    __syncwarp();  // tcgen05.dealloc is warp-collective
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, C::kTmemCols);
+  }
+}
+
+}  // namespace ffn
+}  // namespace ccv

@@ -210,6 +210,8 @@ struct FfnForward {
   const void *w_gate, *w_up, *w_down;
   void* y;
   void* saved;  // h, g, u planes for the backward pass, or null
+  // Where a row length is a multiple of 8 elements its matrices are read by
+  // TMA in place: bases 16-byte aligned, row strides multiples of 8.
 };
 struct FfnBackward {
   FfnShape shape;
@@ -222,7 +224,7 @@ struct FfnBackward {
 };
 // Bytes of one [rows][hidden] plane (rows padded to 16 bytes).
 size_t ffn_plane_bytes(const FfnShape& s);
-size_t ffn_forward_workspace_bytes(const FfnShape& s);
+size_t ffn_forward_workspace_bytes(const FfnShape& s, bool save);
 size_t ffn_backward_workspace_bytes(const FfnShape& s);
 int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream);
 int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream);
@@ -249,6 +251,11 @@ enum TmaSwizzle { kSwizzle64 = 0, kSwizzle128 = 1, kSwizzleNone = 3 };
 int encode_tiled_ex(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
                     const uint64_t* strides_bytes, const uint32_t* box,
                     const uint32_t* elem_strides, TmaSwizzle swizzle, bool elem8);
+
+// Same with the element type named.
+int encode_tiled_typed(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank,
+                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                       const uint32_t* elem_strides, TmaSwizzle swizzle);
 
 // One CTA waits on an mbarrier nothing arrives on; the bounded wait writes
 // CCV_ERR_DEVICE_TIMEOUT into *status_dev (and, with `mirror`, into the

@@ -195,6 +195,14 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
       "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                             int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_commit_group() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -202,6 +210,11 @@ __device__ __forceinline__ void bulk_commit_group() {
 // shared-memory source (the buffer may be rewritten).
 __device__ __forceinline__ void bulk_wait_read_all() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+// Same, allowing the N most recent bulk groups to still be reading.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read_le() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 // Same, allowing the most recent bulk group to still be reading.
 __device__ __forceinline__ void bulk_wait_read_le1() {
@@ -545,6 +558,46 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
       " [%0], %1;" ::"r"(bar),
       "h"(mask)
       : "memory");
+}
+
+// The same pair MMA on 16-bit operands (both f16 or both bf16, as idesc says).
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor for a 16-bit operand stored with its M or N
+// index innermost, 128-byte swizzle: rows of 64 M/N elements (128 bytes), one
+// per K index, so 8 K indexes are a 1024-byte swizzle atom and the next 8
+// follow it (the stride offset); the next 64 M/N elements lie `block_bytes`
+// further (the leading offset).  One K step of 16 advances the address by
+// 2048 bytes.
+__device__ __forceinline__ uint64_t desc_mnmajor_sw128(uint32_t smem_addr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((block_bytes >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((1024u >> 4) & 0x3FFFu) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+// Instruction descriptor for kind::f16, FP32 accumulator.  mn_a / mn_b: the
+// operand's M / N index is innermost (else K).
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, bool bf16, bool mn_a,
+                                                 bool mn_b) {
+  return (1u << 4)                       // D format: F32
+         | ((bf16 ? 1u : 0u) << 7)       // A format: BF16 or F16
+         | ((bf16 ? 1u : 0u) << 10)      // B format
+         | ((mn_a ? 1u : 0u) << 15)      // A major-ness
+         | ((mn_b ? 1u : 0u) << 16)      // B major-ness
+         | ((n >> 3) << 17)              // N / 8
+         | ((m >> 4) << 24);             // M / 16
 }
 
 // Instruction descriptor for kind::tf32, FP32 accumulator, K-major A and B.

@@ -29,6 +29,11 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+template <typename T>
+constexpr bool kIsBf16 = false;
+template <>
+constexpr bool kIsBf16<__nv_bfloat16> = true;
+
 inline size_t dtype_bytes(int dtype) { return dtype == CCV_DTYPE_F32 ? 4 : 2; }
 inline bool valid_dtype(int dtype) {
   return dtype == CCV_DTYPE_F32 || dtype == CCV_DTYPE_BF16 || dtype == CCV_DTYPE_F16;

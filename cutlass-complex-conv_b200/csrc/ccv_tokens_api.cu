@@ -66,6 +66,21 @@ int check_ffn(const FfnShape& s) {
   return rc;
 }
 
+// Rows of `length` elements that TMA reads in place (see FfnForward).
+int check_in_place(const void* p, int64_t length, int64_t stride, const char* msg) {
+  if (length % 8 == 0 && (!aligned_to(p, 16) || stride % 8 != 0)) return invalid(msg);
+  return CCV_OK;
+}
+
+int check_ffn_alignment(const FfnShape& s, const void* x, int64_t x_stride, const void* w_gate,
+                        const void* w_up, const void* w_down) {
+  const char* msg = "rows of a multiple of 8 elements must start at 16-byte boundaries";
+  int rc = check_in_place(x, s.features, s.rows > 1 ? x_stride : 0, msg);
+  if (rc == CCV_OK) rc = check_in_place(w_gate, s.features, 0, msg);
+  if (rc == CCV_OK) rc = check_in_place(w_up, s.features, 0, msg);
+  return rc == CCV_OK ? check_in_place(w_down, s.hidden, 0, msg) : rc;
+}
+
 int check_workspace(const void* ws, size_t have, size_t need) {
   if (need == 0) return CCV_OK;
   if (ws == nullptr || !aligned_to(ws, 256) || have < need) {
@@ -146,18 +161,19 @@ int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, 
 }
 
 size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden) {
-  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
-  return 3 * ffn_plane_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+  const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
+  return check_ffn(s) == CCV_OK ? 3 * ffn_plane_bytes(s) : 0;
 }
 
-size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden) {
-  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
-  return ffn_forward_workspace_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden,
+                                             int save) {
+  const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
+  return check_ffn(s) == CCV_OK ? ffn_forward_workspace_bytes(s, save != 0) : 0;
 }
 
 size_t ccv_gated_ffn_backward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden) {
-  if (rows < 0 || features <= 0 || hidden <= 0) return 0;
-  return ffn_backward_workspace_bytes({rows, features, hidden, CCV_DTYPE_BF16, 0});
+  const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
+  return check_ffn(s) == CCV_OK ? ffn_backward_workspace_bytes(s) : 0;
 }
 
 int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gate,
@@ -166,23 +182,27 @@ int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gat
                           void* saved, size_t saved_bytes, void* workspace,
                           size_t workspace_bytes, ccv_stream_t stream) {
   return guarded([&]() -> int {
-    FfnForward f = {{rows, features, hidden, dtype, activation}, x,      x_row_stride, w_gate, w_up,
-                    w_down,                                      y, saved};
+    FfnForward f = {{rows, features, hidden, dtype, activation},
+                    x, rows > 1 ? x_row_stride : features, w_gate, w_up, w_down, y, saved};
     int rc = check_ffn(f.shape);
     if (rc != CCV_OK || rows == 0) return rc;
     if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr ||
         y == nullptr) {
       return invalid("null tensor pointer");
     }
-    if (x_row_stride < 0) return invalid("row stride must be non-negative");
+    if (rows > 1 && x_row_stride < features) return invalid("row stride below the row length");
     for (const void* p : {x, w_gate, w_up, w_down, static_cast<const void*>(y)}) {
       if (!aligned_to(p, 2)) return invalid("tensor pointers must be aligned to their element");
+    }
+    if ((rc = check_ffn_alignment(f.shape, x, x_row_stride, w_gate, w_up, w_down)) != CCV_OK ||
+        (rc = check_in_place(y, features, 0, "y must be 16-byte aligned")) != CCV_OK) {
+      return rc;
     }
     if (saved != nullptr && (!aligned_to(saved, 256) || saved_bytes < 3 * ffn_plane_bytes(f.shape))) {
       return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");
     }
     if ((rc = check_workspace(workspace, workspace_bytes,
-                              ffn_forward_workspace_bytes(f.shape))) != CCV_OK) {
+                              ffn_forward_workspace_bytes(f.shape, saved != nullptr))) != CCV_OK) {
       return rc;
     }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -199,7 +219,8 @@ int ccv_gated_ffn_backward(const void* dy, int64_t dy_row_stride, const void* x,
                            size_t workspace_bytes, ccv_stream_t stream) {
   return guarded([&]() -> int {
     FfnBackward b = {{rows, features, hidden, dtype, activation},
-                     dy, dy_row_stride, x, x_row_stride, w_gate, w_up, w_down, saved,
+                     dy, rows > 1 ? dy_row_stride : features,
+                     x, rows > 1 ? x_row_stride : features, w_gate, w_up, w_down, saved,
                      dx, dw_gate, dw_up, dw_down};
     int rc = check_ffn(b.shape);
     if (rc != CCV_OK) return rc;
@@ -210,11 +231,27 @@ int ccv_gated_ffn_backward(const void* dy, int64_t dy_row_stride, const void* x,
         (rows > 0 && (dy == nullptr || x == nullptr || saved == nullptr))) {
       return invalid("null tensor pointer");
     }
-    if (x_row_stride < 0 || dy_row_stride < 0) return invalid("row stride must be non-negative");
+    if (rows > 1 && (x_row_stride < features || dy_row_stride < features)) {
+      return invalid("row stride below the row length");
+    }
     for (const void* p : {dy, x, w_gate, w_up, w_down, static_cast<const void*>(dx),
                           static_cast<const void*>(dw_gate), static_cast<const void*>(dw_up),
                           static_cast<const void*>(dw_down)}) {
       if (!aligned_to(p, 2)) return invalid("tensor pointers must be aligned to their element");
+    }
+    if ((rc = check_ffn_alignment(b.shape, x, x_row_stride, w_gate, w_up, w_down)) != CCV_OK ||
+        (rc = check_in_place(dy, features, rows > 1 ? dy_row_stride : 0,
+                             "dy must be 16-byte aligned")) != CCV_OK) {
+      return rc;
+    }
+    for (const void* p : {static_cast<const void*>(dx), static_cast<const void*>(dw_gate),
+                          static_cast<const void*>(dw_up)}) {
+      if ((rc = check_in_place(p, features, 0, "gradients must be 16-byte aligned")) != CCV_OK) {
+        return rc;
+      }
+    }
+    if ((rc = check_in_place(dw_down, hidden, 0, "gradients must be 16-byte aligned")) != CCV_OK) {
+      return rc;
     }
     if (rows > 0 && (!aligned_to(saved, 256) || saved_bytes < 3 * ffn_plane_bytes(b.shape))) {
       return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");

@@ -287,9 +287,14 @@ int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, 
  * saved (null for inference): ccv_gated_ffn_saved_bytes(), 256-byte aligned,
  * filled with what the backward pass reads (an opaque layout).  The
  * intermediate rows are rounded to 16 bits once each, as operands of the
- * next product. */
+ * next product.  Where features (x, w_gate, w_up, y and their gradients) or
+ * hidden (w_down and its gradient) is a multiple of 8, those matrices are
+ * read and written in place by TMA: 16-byte aligned bases, row strides
+ * multiples of 8.  Others are copied to padded rows in the workspace.
+ * workspace: 256-byte aligned; save != 0 in its query when saved is given. */
 size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden);
-size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden);
+size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden,
+                                             int save);
 int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gate,
                           const void* w_up, const void* w_down, void* y, int dtype,
                           int activation, int64_t rows, int64_t features, int64_t hidden,
