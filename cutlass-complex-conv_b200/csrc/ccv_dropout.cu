@@ -9,6 +9,7 @@
 // The mask is a function of (seed, offset, i): the backward pass is the same
 // call on the gradient, and nothing is stored.
 #include <cmath>
+#include <type_traits>
 
 #include "ccv_internal.h"
 #include "ccv_ptx.cuh"
@@ -31,51 +32,99 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
   return c;
 }
 
-// One thread per group of eight elements.
-template <typename Tx, typename Tr>
-__global__ void dropout_groups(const Tx* __restrict__ x, const Tr* __restrict__ residual,
-                               Tr* __restrict__ y, int64_t count, uint32_t threshold, float scale,
-                               uint64_t seed, uint64_t offset,
-                               const int64_t* __restrict__ offset_dev) {
+constexpr int kUnroll = 4;
+constexpr int kDropoutThreads = 256;
+
+// A thread takes kUnroll groups of eight elements, a block's width apart:
+// the loads of all of them are in flight while their counters are hashed.
+// VEC: x, residual and y are 16-byte aligned.
+template <typename Tx, typename Tr, bool RESIDUAL, bool VEC>
+__global__ void __launch_bounds__(kDropoutThreads)
+    dropout_groups(const Tx* __restrict__ x, const Tr* __restrict__ residual, Tr* __restrict__ y,
+                   int64_t count, uint32_t threshold, float scale, uint64_t seed, uint64_t offset,
+                   const int64_t* __restrict__ offset_dev) {
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   if (offset_dev != nullptr) offset = static_cast<uint64_t>(*offset_dev);
   const uint2 key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
-  const int64_t groups = (count + 7) / 8;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t g = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups;
-       g += step) {
+  const int64_t first =
+      static_cast<int64_t>(blockIdx.x) * (kDropoutThreads * kUnroll) + threadIdx.x;
+  Vec<Tx, 8> vx[kUnroll];
+  Vec<Tr, 8> vr[kUnroll];
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+    const int64_t i = (first + k * kDropoutThreads) * 8;
+    if (VEC && i + 8 <= count) {
+      vx[k] = load_vec<Tx, 8>(x + i);
+      if (RESIDUAL) vr[k] = load_vec<Tr, 8>(residual + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (i + j < count) {
+          vx[k].e[j] = x[i + j];
+          if (RESIDUAL) vr[k].e[j] = residual[i + j];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kUnroll; ++k) {
+    const int64_t g = first + k * kDropoutThreads;
+    const int64_t i = g * 8;
+    if (i >= count) break;
     const uint4 r = philox4x32_10(
         make_uint4(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32),
                    static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
         key);
     const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+    float o[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int64_t i = g * 8 + j;
-      if (i < count) {
-        const uint32_t part = (word[j / 2] >> (16 * (j & 1))) & 0xffffu;
-        float v = part >= threshold ? to_f32(x[i]) * scale : 0.f;
-        if (residual != nullptr) v += to_f32(residual[i]);
-        y[i] = from_f32<Tr>(v);
+      const uint32_t part = (j & 1) != 0 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
+      o[j] = part >= threshold ? to_f32(vx[k].e[j]) * scale : 0.f;
+      if (RESIDUAL) o[j] += to_f32(vr[k].e[j]);
+    }
+    if (VEC && i + 8 <= count) {
+      store_vec<Tr, 8>(y + i, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (i + j < count) y[i + j] = from_f32<Tr>(o[j]);
       }
     }
   }
 }
 
-template <typename Tx, typename Tr>
-int run_dropout(const Dropout& a, cudaStream_t stream) {
+template <typename Tx, typename Tr, bool RESIDUAL, bool VEC>
+int launch_groups(const Dropout& a, cudaStream_t stream) {
   const uint32_t threshold = static_cast<uint32_t>(std::floor(a.p * 65536.0 + 0.5));
   const float scale =
       threshold >= 65536u ? 0.f : static_cast<float>(65536.0 / (65536.0 - threshold));
-  const int64_t blocks64 = ((a.count + 7) / 8 + 255) / 256;
-  const unsigned blocks = static_cast<unsigned>(blocks64 < 148 * 16 ? blocks64 : 148 * 16);
+  constexpr int64_t per_block = 8LL * kDropoutThreads * kUnroll;
+  const int64_t blocks = (a.count + per_block - 1) / per_block;
   return launched(
-      launch_kernel(dropout_groups<Tx, Tr>, dim3(blocks), dim3(256), 0, stream, 1,
-                    static_cast<const Tx*>(a.x), static_cast<const Tr*>(a.residual),
-                    static_cast<Tr*>(a.y), a.count, threshold, scale, a.seed, a.offset,
-                    a.offset_dev),
+      launch_kernel(dropout_groups<Tx, Tr, RESIDUAL, VEC>, dim3(static_cast<unsigned>(blocks)),
+                    dim3(kDropoutThreads), 0, stream, 1, static_cast<const Tx*>(a.x),
+                    static_cast<const Tr*>(a.residual), static_cast<Tr*>(a.y), a.count, threshold,
+                    scale, a.seed, a.offset, a.offset_dev),
       "dropout");
+}
+
+template <typename Tx, typename Tr>
+int run_dropout(const Dropout& a, cudaStream_t stream) {
+  const bool vec = vec_rows<Tx, 8>(a.x, 0, 8) && vec_rows<Tr, 8>(a.y, 0, 8) &&
+                   vec_rows<Tr, 8>(a.residual, 0, 8);
+  if (a.residual != nullptr) {
+    return vec ? launch_groups<Tx, Tr, true, true>(a, stream)
+               : launch_groups<Tx, Tr, true, false>(a, stream);
+  }
+  // Without a residual the output has the input's type (checked by the entry).
+  if constexpr (std::is_same_v<Tx, Tr>) {
+    return vec ? launch_groups<Tx, Tr, false, true>(a, stream)
+               : launch_groups<Tx, Tr, false, false>(a, stream);
+  } else {
+    return CCV_ERR_INVALID_ARGUMENT;
+  }
 }
 
 }  // namespace

@@ -18,6 +18,7 @@
 #include <mutex>
 
 #include "ccv_ffn_gemm.cuh"
+#include "ccv_ffn_rows.cuh"
 #include "ccv_internal.h"
 #include "ccv_ptx.cuh"
 #include "ccv_tokens.cuh"
@@ -105,6 +106,75 @@ __global__ void ffn_split_sum(const SplitSums p) {
       if (c + j < s.n) o[j] = from_f32<T>(f[j]);
     }
   }
+}
+
+// ------------------------------------------------------------ few rows
+// Up to this many rows the block streams its weights through mma.sync.
+constexpr int64_t kFewRows = 16;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, int NT>
+int launch_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t stream) {
+  const FfnShape& s = f.shape;
+  const int64_t sms = device_sm_count(), fp = padded(s.hidden);
+  ffn::RowsParams p = {};
+  p.x = static_cast<const uint16_t*>(f.x);
+  p.x_stride = f.x_stride;
+  p.w0 = static_cast<const uint16_t*>(f.w_gate);
+  p.w1 = static_cast<const uint16_t*>(f.w_up);
+  p.out = static_cast<uint16_t*>(h);
+  p.g = static_cast<uint16_t*>(g);
+  p.u = static_cast<uint16_t*>(u);
+  p.out_stride = fp;
+  p.rows = static_cast<int>(s.rows);
+  p.k = static_cast<int>(s.features);
+  p.outputs = static_cast<int>(s.hidden);
+  p.act = s.activation;
+  // Groups of 8 outputs per block: as many as leave four blocks per SM.
+  const int64_t groups = (s.hidden + 7) / 8;
+  p.blocks_per_cta = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, groups / (4 * sms))));
+  const bool vec = s.features % 8 == 0 && aligned16(f.x) && f.x_stride % 8 == 0 &&
+                   aligned16(f.w_gate) && aligned16(f.w_up);
+  const dim3 gate_grid(static_cast<unsigned>((groups + p.blocks_per_cta - 1) / p.blocks_per_cta));
+  int rc = launched(
+      vec ? launch_kernel(ffn::ffn_rows_gate<T, NT, true>, gate_grid, dim3(ffn::kRowsThreads), 0,
+                          stream, 1, p)
+          : launch_kernel(ffn::ffn_rows_gate<T, NT, false>, gate_grid, dim3(ffn::kRowsThreads), 0,
+                          stream, 1, p),
+      "gated feed-forward gate");
+  if (rc != CCV_OK) return rc;
+  ffn::RowsParams d = {};
+  d.x = static_cast<const uint16_t*>(h);
+  d.x_stride = fp;
+  d.w0 = static_cast<const uint16_t*>(f.w_down);
+  d.out = static_cast<uint16_t*>(f.y);
+  d.out_stride = s.features;
+  d.rows = p.rows;
+  d.k = p.outputs;
+  d.outputs = p.k;
+  // Blocks per cluster: enough for two blocks per SM, while each warp keeps
+  // two chunks of the reduction.
+  const int64_t tiles = (s.features + 15) / 16;
+  int cluster = 1;
+  while (cluster < 8 && tiles * cluster < 2 * sms &&
+         s.hidden >= static_cast<int64_t>(2 * cluster) * ffn::kRowsWarps * 2 * ffn::kChunk) {
+    cluster *= 2;
+  }
+  const dim3 down_grid(static_cast<unsigned>(tiles * cluster));
+  const bool vec_w = s.hidden % 8 == 0 && aligned16(f.w_down);
+  return launched(
+      vec_w ? launch_kernel(ffn::ffn_rows_down<T, NT, true>, down_grid, dim3(ffn::kRowsThreads), 0,
+                            stream, cluster, d)
+            : launch_kernel(ffn::ffn_rows_down<T, NT, false>, down_grid, dim3(ffn::kRowsThreads), 0,
+                            stream, cluster, d),
+      "gated feed-forward down");
+}
+
+template <typename T>
+int run_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t stream) {
+  return f.shape.rows <= 8 ? launch_rows<T, 1>(f, h, g, u, stream)
+                           : launch_rows<T, 2>(f, h, g, u, stream);
 }
 
 // ------------------------------------------------------------ planning
@@ -312,7 +382,7 @@ void* take_rows(Carver& c, int64_t rows, int64_t cols) {
 }
 
 struct ForwardPlan {
-  bool pad_d, pad_f;
+  bool pad_d = false, pad_f = false;
   Plan gate, down;
   void *h = nullptr, *x = nullptr, *w_gate = nullptr, *w_up = nullptr, *w_down = nullptr,
        *y = nullptr, *partial = nullptr;
@@ -320,6 +390,10 @@ struct ForwardPlan {
 
 ForwardPlan plan_forward(const FfnShape& s, bool save, Carver& c) {
   ForwardPlan p;
+  if (s.rows <= kFewRows) {
+    if (!save) p.h = take_rows(c, s.rows, s.hidden);
+    return p;
+  }
   p.pad_d = s.features % 8 != 0;
   p.pad_f = s.hidden % 8 != 0;
   const Extent eh = {s.rows, s.hidden}, ey = {s.rows, s.features};
@@ -404,6 +478,13 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   const size_t plane = ffn_plane_bytes(s);
   Carver c{static_cast<char*>(ws)};
   const ForwardPlan p = plan_forward(s, saved != nullptr, c);
+  if (m <= kFewRows) {
+    void* h = saved != nullptr ? saved : p.h;
+    void* g = saved != nullptr ? saved + plane : nullptr;
+    void* u = saved != nullptr ? saved + 2 * plane : nullptr;
+    return s.dtype == CCV_DTYPE_BF16 ? run_rows<__nv_bfloat16>(f, h, g, u, stream)
+                                     : run_rows<__half>(f, h, g, u, stream);
+  }
   const Padded x{f.x, f.x_stride, m, d, p.x}, wg{f.w_gate, d, hid, d, p.w_gate},
       wu{f.w_up, d, hid, d, p.w_up}, wd{f.w_down, hid, d, hid, p.w_down};
   for (const Padded* q : {&x, &wg, &wu, &wd}) {
