@@ -70,41 +70,47 @@ int copy_rows(const void* src, int64_t src_pitch, void* dst, int64_t dst_pitch, 
 }
 
 struct SplitSum {
-  const float* partial;  // [splits][m][np]
-  void* out;
-  int64_t m, n, np, ldo;
-};
-struct SplitSums {
-  SplitSum s[ffn::kMaxProblems];
-  int splits;
+  const float* partial;  // [split tile][split][256][bn]
+  ffn::Tiles tiles[ffn::kMaxProblems];
+  void* out[ffn::kMaxProblems];
+  int64_t ldo[ffn::kMaxProblems];
+  int problems, whole, splits, bn;
 };
 
-// out = sum over the splits, in split order; four columns per thread.
+// The split tiles' results: their parts added in order, four columns per
+// thread; blockIdx.y is the tile.
 template <typename T>
-__global__ void ffn_split_sum(const SplitSums p) {
+__global__ void __launch_bounds__(256) ffn_split_sum(const SplitSum p) {
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  const SplitSum& s = p.s[blockIdx.y];
-  const int64_t quads = s.np / 4;
-  const int64_t total = s.m * quads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t m = i / quads, c = (i - m * quads) * 4;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < p.splits; ++k) {
-      const float4 v =
-          *reinterpret_cast<const float4*>(s.partial + (k * s.m + m) * s.np + c);
-      a.x += v.x;
-      a.y += v.y;
-      a.z += v.z;
-      a.w += v.w;
-    }
-    T* o = static_cast<T*>(s.out) + m * s.ldo + c;
-    const float f[4] = {a.x, a.y, a.z, a.w};
+  int problem, tm, tn;
+  ffn::locate(p.tiles, p.problems, p.whole + static_cast<int>(blockIdx.y), problem, tm, tn);
+  const int quads = p.bn / 4;
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  const int r = i / quads, c = (i - r * quads) * 4;
+  const int64_t row = static_cast<int64_t>(tm) * 256 + r, col = static_cast<int64_t>(tn) * p.bn + c;
+  const ffn::Tiles& t = p.tiles[problem];
+  if (row >= t.m || col >= t.n) return;
+  const int64_t part = 256LL * p.bn;
+  const float* src = p.partial + blockIdx.y * part * p.splits + static_cast<int64_t>(r) * p.bn + c;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < p.splits; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(src + k * part);
+    a.x += v.x;
+    a.y += v.y;
+    a.z += v.z;
+    a.w += v.w;
+  }
+  T* o = static_cast<T*>(p.out[problem]) + row * p.ldo[problem] + col;
+  const float f[4] = {a.x, a.y, a.z, a.w};
+  if (p.ldo[problem] % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & 7) == 0 && col + 4 <= t.n) {
+    store_vec<T, 4>(o, f);
+    return;
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (c + j < s.n) o[j] = from_f32<T>(f[j]);
-    }
+  for (int j = 0; j < 4; ++j) {
+    if (col + j < t.n) o[j] = from_f32<T>(f[j]);
   }
 }
 
@@ -184,7 +190,12 @@ struct Extent {
 
 struct Plan {
   int bn = 256;
+  int64_t whole = 0;   // tiles that one unit computes
+  int64_t tail = 0;    // the others, in `splits` parts each
   int splits = 1;
+  size_t partial_bytes() const {
+    return static_cast<size_t>(tail) * splits * 256 * bn * sizeof(float);
+  }
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -195,29 +206,37 @@ int64_t tile_count(const Extent* e, int problems, int width) {
   return t;
 }
 
-// Tile width and reduction split by an estimate in clocks: a K step of a
-// 256 x BN tile is 2 BN clocks of multiplication at full rate, the narrower
-// tile loses some of it to its larger share of loads; a unit has a fixed
-// start and end; a split writes and sums partial results.
+// Tile width, and the split of the tiles past the last full wave, by an
+// estimate in clocks.  A K step of a 256 x 256 tile is 512 clocks of
+// multiplication; of a 256 x 128 tile it measured 0.85 times that on B200,
+// not half, because the narrower tile reads as much of A from shared memory
+// (128 bytes a clock is all there is).  Tiles that fill whole waves of the
+// clusters are never split; the rest may be, so that the last wave is short,
+// at the cost of a second launch and of the partial sums' traffic.
 Plan make_plan(const Extent* e, int problems, int64_t ksteps, bool may_split, bool gate) {
   const int64_t clusters = std::max(1, device_sm_count() / 2);
   Plan best;
   double best_cost = 1e30;
   for (int bn : {256, 128}) {
     const int64_t tiles = tile_count(e, problems, gate ? bn / 2 : bn);
-    const double step = bn == 256 ? 512.0 : 290.0;
-    for (int splits = 1; splits <= (may_split ? 64 : 1) && splits <= ksteps; ++splits) {
-      const double waves = static_cast<double>(ceil_div(tiles * splits, clusters));
-      double cost = waves * (static_cast<double>(ceil_div(ksteps, splits)) * step + 600.0);
-      if (splits > 1) {
-        double bytes = 0;
-        for (int i = 0; i < problems; ++i) bytes += 8.0 * e[i].m * e[i].n * splits;
-        cost += 4000.0 + bytes / 3500.0;
+    const double step = bn == 256 ? 512.0 : 435.0;
+    const int64_t full = tiles / clusters * clusters;
+    const int64_t rest = tiles - full;
+    const double base = static_cast<double>(full / clusters) * ksteps * step;
+    const int most = rest > 0 && may_split ? static_cast<int>(std::min<int64_t>(64, ksteps)) : 1;
+    for (int splits = 1; splits <= most; ++splits) {
+      double cost = base;
+      if (rest > 0) {
+        cost += static_cast<double>(ceil_div(rest * splits, clusters) * ceil_div(ksteps, splits)) *
+                step;
       }
+      if (splits > 1) cost += 5000.0 + 8.0 * rest * splits * 256 * bn / 3500.0;
       if (cost < best_cost * 0.999) {
         best_cost = cost;
         best.bn = bn;
         best.splits = splits;
+        best.whole = splits > 1 ? full : tiles;
+        best.tail = splits > 1 ? rest : 0;
       }
     }
   }
@@ -292,8 +311,9 @@ template <int MODE, bool A_MN, bool B_MN>
 struct Product {
   GemmParams prm = {};
   Plan plan;
+  SplitSum sums = {};
   int dtype;
-  int64_t units = 0;
+  int64_t tiles = 0;
   int rc = CCV_OK;
 
   Product(int dtype_, const Plan& plan_, int64_t k, int act) : plan(plan_), dtype(dtype_) {
@@ -302,6 +322,7 @@ struct Product {
     prm.segments = 1;
     prm.ksteps = static_cast<int>(ceil_div(k, ffn::kStepK));
     prm.splits = plan.splits;
+    prm.whole = static_cast<int>(plan.whole);
     prm.act = act;
   }
   void operand_a(int i, const Matrix& x) {
@@ -316,19 +337,21 @@ struct Product {
     }
   }
   void result(int i, void* base, int64_t m, int64_t n, int64_t ld) {
-    if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, MODE == ffn::GATE ? 32 : 64, 32);
+    if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, MODE == ffn::PLAIN ? 64 : 32, 32);
+    sums.out[i] = base;
+    sums.ldo[i] = ld;
   }
-  void partials(int i, void* base, int64_t m, int64_t n) {
-    const uint64_t np = static_cast<uint64_t>((n + 3) / 4 * 4);
-    const uint64_t dims[3] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m),
-                              static_cast<uint64_t>(plan.splits)};
-    const uint64_t strides[2] = {np * 4, np * 4 * static_cast<uint64_t>(m)};
+  // Storage for the split tiles' parts (none without a split).
+  void partials(void* base) {
+    if (plan.tail == 0 || rc != CCV_OK) return;
+    const uint64_t bn = static_cast<uint64_t>(plan.bn);
+    const uint64_t dims[3] = {bn, 256, static_cast<uint64_t>(plan.tail * plan.splits)};
+    const uint64_t strides[2] = {bn * 4, bn * 4 * 256};
     const uint32_t box[3] = {32, 32, 1};
     const uint32_t es[3] = {1, 1, 1};
-    if (rc == CCV_OK) {
-      rc = encode_tiled_typed(&prm.out[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, 3, dims, strides,
-                              box, es, kSwizzle128);
-    }
+    sums.partial = static_cast<const float*>(base);
+    rc = encode_tiled_typed(&prm.partial, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, 3, dims, strides,
+                            box, es, kSwizzle128);
   }
   void problem(int i, int64_t m, int64_t n) {
     ffn::Tiles& t = prm.tiles[i];
@@ -336,33 +359,34 @@ struct Product {
     t.n = static_cast<int>(n);
     t.tiles_m = static_cast<int>(ceil_div(m, 256));
     t.tiles_n = static_cast<int>(ceil_div(n, MODE == ffn::GATE ? plan.bn / 2 : plan.bn));
-    t.first = static_cast<int>(units);
-    units += static_cast<int64_t>(t.tiles_m) * t.tiles_n * plan.splits;
+    t.first = static_cast<int>(tiles);
+    tiles += static_cast<int64_t>(t.tiles_m) * t.tiles_n;
     prm.problems = i + 1;
   }
   int launch(cudaStream_t stream) {
     if (rc != CCV_OK) return rc;
     if (prm.status == nullptr) return CCV_ERR_DEVICE;
+    // Fewer problems than planned for leave fewer tiles.
+    prm.whole = static_cast<int>(std::min<int64_t>(plan.whole, tiles));
+    const int64_t tail = tiles - prm.whole;
+    const int64_t units = prm.whole + tail * plan.splits;
     if (units > 0x7fffffff) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
     prm.units = static_cast<int>(units);
-    return launch_product<MODE, A_MN, B_MN>(prm, dtype, plan.bn, stream);
+    const int launched_rc = launch_product<MODE, A_MN, B_MN>(prm, dtype, plan.bn, stream);
+    if (launched_rc != CCV_OK || tail == 0) return launched_rc;
+    for (int i = 0; i < prm.problems; ++i) sums.tiles[i] = prm.tiles[i];
+    sums.problems = prm.problems;
+    sums.whole = prm.whole;
+    sums.splits = plan.splits;
+    sums.bn = plan.bn;
+    const dim3 grid(static_cast<unsigned>(plan.bn / 4), static_cast<unsigned>(tail));
+    return launched(
+        dtype == CCV_DTYPE_BF16
+            ? launch_kernel(ffn_split_sum<__nv_bfloat16>, grid, dim3(256), 0, stream, 1, sums)
+            : launch_kernel(ffn_split_sum<__half>, grid, dim3(256), 0, stream, 1, sums),
+        "gated feed-forward split sum");
   }
 };
-
-size_t partial_bytes(const Plan& p, const Extent& e) {
-  return p.splits > 1 ? static_cast<size_t>(p.splits) * e.m * ((e.n + 3) / 4 * 4) * 4 : 0;
-}
-
-int split_sum(const SplitSums& sums, int problems, int dtype, cudaStream_t stream) {
-  int64_t most = 0;
-  for (int i = 0; i < problems; ++i) most = std::max(most, sums.s[i].m * (sums.s[i].np / 4));
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(most, 256), 148 * 8));
-  const dim3 grid(blocks, problems);
-  return launched(dtype == CCV_DTYPE_BF16
-                      ? launch_kernel(ffn_split_sum<__nv_bfloat16>, grid, dim3(256), 0, stream, 1, sums)
-                      : launch_kernel(ffn_split_sum<__half>, grid, dim3(256), 0, stream, 1, sums),
-                  "gated feed-forward split sum");
-}
 
 // A [rows][cols] operand with rows TMA can read: itself, or its padded copy.
 struct Padded {
@@ -404,10 +428,10 @@ ForwardPlan plan_forward(const FfnShape& s, bool save, Carver& c) {
     p.x = take_rows(c, s.rows, s.features);
     p.w_gate = take_rows(c, s.hidden, s.features);
     p.w_up = take_rows(c, s.hidden, s.features);
-    if (p.down.splits == 1) p.y = take_rows(c, s.rows, s.features);
+    p.y = take_rows(c, s.rows, s.features);
   }
   if (p.pad_f) p.w_down = take_rows(c, s.features, s.hidden);
-  if (p.down.splits > 1) p.partial = c.take(partial_bytes(p.down, ey));
+  p.partial = c.take(p.down.partial_bytes());
   return p;
 }
 
@@ -436,20 +460,13 @@ BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
     p.x = take_rows(c, s.rows, s.features);
     p.w_gate = take_rows(c, s.hidden, s.features);
     p.w_up = take_rows(c, s.hidden, s.features);
-    if (p.dx.splits == 1) p.out_dx = take_rows(c, s.rows, s.features);
+    p.out_dx = take_rows(c, s.rows, s.features);
   }
   if (p.pad_f) p.w_down = take_rows(c, s.features, s.hidden);
-  size_t partial = partial_bytes(p.dx, ex), dw = 0;
   for (int i = 0; i < 3; ++i) {
-    if (p.dw.splits == 1) {
-      if (i < 2 ? p.pad_d : p.pad_f) {
-        p.out_dw[i] = take_rows(c, p.dw_extent[i].m, p.dw_extent[i].n);
-      }
-    } else {
-      dw += align256(partial_bytes(p.dw, p.dw_extent[i]));
-    }
+    if (i < 2 ? p.pad_d : p.pad_f) p.out_dw[i] = take_rows(c, p.dw_extent[i].m, p.dw_extent[i].n);
   }
-  p.partial = c.take(std::max(partial, dw));
+  p.partial = c.take(std::max(p.dx.partial_bytes(), p.dw.partial_bytes()));
   return p;
 }
 
@@ -511,15 +528,7 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   y.operand_a(0, {h, hid, m, fp});
   y.operand_b(0, wd.matrix());
   y.problem(0, m, d);
-  if (p.down.splits > 1) {
-    y.partials(0, p.partial, m, d);
-    const int rc = y.launch(stream);
-    if (rc != CCV_OK) return rc;
-    SplitSums sums = {};
-    sums.splits = p.down.splits;
-    sums.s[0] = {static_cast<const float*>(p.partial), f.y, m, d, (d + 3) / 4 * 4, d};
-    return split_sum(sums, 1, s.dtype, stream);
-  }
+  y.partials(p.partial);
   y.result(0, p.y != nullptr ? p.y : f.y, m, d, p.y != nullptr ? padded(d) : d);
   const int rc = y.launch(stream);
   if (rc != CCV_OK || p.y == nullptr) return rc;
@@ -560,7 +569,7 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
     g.result(0, p.dg, m, hid, fp);
     g.result(1, p.du, m, hid, fp);
     for (int i = 0; i < 2 && g.rc == CCV_OK; ++i) {
-      g.rc = encode_2d(&g.prm.in[i], s.dtype, saved + (i + 1) * plane, hid, m, fp, 64, 32);
+      g.rc = encode_2d(&g.prm.in[i], s.dtype, saved + (i + 1) * plane, hid, m, fp, 32, 32);
     }
     g.problem(0, m, hid);
     if ((rc = g.launch(stream)) != CCV_OK) return rc;
@@ -573,50 +582,31 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
     g.operand_b(0, wg.matrix());
     g.operand_b(1, wu.matrix());
     g.problem(0, m, d);
-    if (p.dx.splits > 1) {
-      g.partials(0, p.partial, m, d);
-      if ((rc = g.launch(stream)) != CCV_OK) return rc;
-      SplitSums sums = {};
-      sums.splits = p.dx.splits;
-      sums.s[0] = {static_cast<const float*>(p.partial), b.dx, m, d, (d + 3) / 4 * 4, d};
-      if ((rc = split_sum(sums, 1, s.dtype, stream)) != CCV_OK) return rc;
-    } else {
-      void* out = p.out_dx != nullptr ? p.out_dx : b.dx;
-      g.result(0, out, m, d, p.out_dx != nullptr ? padded(d) : d);
-      if ((rc = g.launch(stream)) != CCV_OK) return rc;
-      if (p.out_dx != nullptr &&
-          (rc = copy_rows(out, padded(d), b.dx, d, m, d, stream)) != CCV_OK) {
-        return rc;
-      }
+    void* out = p.out_dx != nullptr ? p.out_dx : b.dx;
+    g.result(0, out, m, d, p.out_dx != nullptr ? padded(d) : d);
+    g.partials(p.partial);
+    if ((rc = g.launch(stream)) != CCV_OK) return rc;
+    if (p.out_dx != nullptr && (rc = copy_rows(out, padded(d), b.dx, d, m, d, stream)) != CCV_OK) {
+      return rc;
     }
   }
   const Matrix left[3] = {{p.dg, hid, m, fp}, {p.du, hid, m, fp}, dy.matrix()};
   const Matrix right[3] = {x.matrix(), x.matrix(), {saved, hid, m, fp}};
   Product<ffn::PLAIN, true, true> g(s.dtype, p.dw, m, 0);
-  SplitSums sums = {};
-  sums.splits = p.dw.splits;
   int count = 0;
-  char* partial = static_cast<char*>(p.partial);
   for (int i = 0; i < 3; ++i) {
     if (dw[i] == nullptr) continue;
     const Extent& e = p.dw_extent[i];
     g.operand_a(count, left[i]);
     g.operand_b(count, right[i]);
     g.problem(count, e.m, e.n);
-    if (p.dw.splits > 1) {
-      g.partials(count, partial, e.m, e.n);
-      sums.s[count] = {reinterpret_cast<const float*>(partial), dw[i], e.m, e.n, (e.n + 3) / 4 * 4,
-                       e.n};
-      partial += align256(partial_bytes(p.dw, e));
-    } else {
-      void* out = p.out_dw[i] != nullptr ? p.out_dw[i] : dw[i];
-      g.result(count, out, e.m, e.n, p.out_dw[i] != nullptr ? padded(e.n) : e.n);
-    }
+    void* out = p.out_dw[i] != nullptr ? p.out_dw[i] : dw[i];
+    g.result(count, out, e.m, e.n, p.out_dw[i] != nullptr ? padded(e.n) : e.n);
     ++count;
   }
   if (count == 0) return CCV_OK;
+  g.partials(p.partial);
   if ((rc = g.launch(stream)) != CCV_OK) return rc;
-  if (p.dw.splits > 1) return split_sum(sums, count, s.dtype, stream);
   for (int i = 0; i < 3; ++i) {
     if (dw[i] == nullptr || p.out_dw[i] == nullptr) continue;
     const Extent& e = p.dw_extent[i];

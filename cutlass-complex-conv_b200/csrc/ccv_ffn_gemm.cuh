@@ -48,7 +48,7 @@ constexpr int kTimeoutCode = CCV_ERR_DEVICE_TIMEOUT;
 struct Tiles {
   int m, n;              // extents of the result
   int tiles_m, tiles_n;
-  int first;             // first work unit
+  int first;             // first tile
 };
 
 struct alignas(64) GemmParams {
@@ -57,11 +57,14 @@ struct alignas(64) GemmParams {
   CUtensorMap a[kMaxProblems], b[kMaxProblems];
   CUtensorMap out[kMaxProblems];  // GATE: h, g, u; GRAD: dg, du; PLAIN: per problem
   CUtensorMap in[2];              // GRAD: g, u
+  CUtensorMap partial;            // split tiles: fp32 [tile part][256][BN]
   Tiles tiles[kMaxProblems];
   int* status;
   int problems, segments;
   int ksteps;   // per segment
-  int splits;   // PLAIN: parts of the reduction, summed by ffn_split_sum
+  // Work units: tiles 0 .. whole - 1, then the other tiles in `splits` parts
+  // of the reduction each (PLAIN), whose partial sums ffn_split_sum adds.
+  int whole, splits;
   int units;
   int save;     // GATE: store g and u too
   int act;
@@ -79,49 +82,75 @@ struct Config {
   static constexpr int kSmem = kBarOffset + kBarBytes + 1024;
   static constexpr int kTmemCols = 2 * BN;
   static_assert(kSmem <= 232448, "shared memory");
-  static_assert((2 * kStages + 5 + kEpiWarps) * 8 + 16 <= kBarBytes, "barriers");
+  static_assert((2 * kStages + 5 + 2 * kEpiWarps) * 8 + 16 <= kBarBytes, "barriers");
 };
 
 struct Unit {
-  int problem, tm, tn, split, k0, k1;
+  int problem, tm, tn, k0, k1;
+  int part;  // index among the split tiles' parts, -1: a whole tile
 };
+
+// Problem, tile row and tile column of a tile.
+__host__ __device__ __forceinline__ void locate(const Tiles* tiles, int problems, int tile,
+                                                int& problem, int& tm, int& tn) {
+  problem = 0;
+  for (int i = 1; i < kMaxProblems; ++i) {
+    if (i < problems && tile >= tiles[i].first) problem = i;
+  }
+  const Tiles& t = tiles[problem];
+  const int local = tile - t.first;
+  // Bands of kRasterRows tile rows, walked column by column.
+  const int band = local / (kRasterRows * t.tiles_n);
+  const int r = local - band * kRasterRows * t.tiles_n;
+  const int left = t.tiles_m - band * kRasterRows;
+  const int rows = left < kRasterRows ? left : kRasterRows;
+  tn = r / rows;
+  tm = band * kRasterRows + (r - tn * rows);
+}
 
 __device__ __forceinline__ Unit decode(const GemmParams& p, int u) {
   Unit w;
-  w.problem = 0;
-#pragma unroll
-  for (int i = 1; i < kMaxProblems; ++i) {
-    if (i < p.problems && u >= p.tiles[i].first) w.problem = i;
-  }
-  const Tiles& t = p.tiles[w.problem];
-  const int local = u - t.first;
-  const int tile = local / p.splits;
-  w.split = local - tile * p.splits;
-  // Bands of kRasterRows tile rows, walked column by column.
-  const int band = tile / (kRasterRows * t.tiles_n);
-  const int r = tile - band * kRasterRows * t.tiles_n;
-  const int rows = min(kRasterRows, t.tiles_m - band * kRasterRows);
-  w.tn = r / rows;
-  w.tm = band * kRasterRows + (r - w.tn * rows);
   const int total = p.ksteps * p.segments;
-  w.k0 = static_cast<int>(static_cast<long long>(total) * w.split / p.splits);
-  w.k1 = static_cast<int>(static_cast<long long>(total) * (w.split + 1) / p.splits);
+  int tile = u;
+  w.part = -1;
+  w.k0 = 0;
+  w.k1 = total;
+  if (u >= p.whole) {
+    w.part = u - p.whole;
+    const int q = w.part / p.splits;
+    const int s = w.part - q * p.splits;
+    tile = p.whole + q;
+    w.k0 = static_cast<int>(static_cast<long long>(total) * s / p.splits);
+    w.k1 = static_cast<int>(static_cast<long long>(total) * (s + 1) / p.splits);
+  }
+  locate(p.tiles, p.problems, tile, w.problem, w.tm, w.tn);
   return w;
 }
 
-// act(g): the sigmoid from the hardware exponential and reciprocal.  GELU's
-// normal distribution is Abramowitz and Stegun 7.1.26 (|error of erf| <=
-// 1.5e-7), a polynomial times exp(-g^2/2), the exponential its slope needs
-// too.  Both errors lie far below the 16-bit rounding of the result.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(g) and act'(g).  The sigmoid is two hardware approximations (2^x and
+// 1/x, a few 2^-23 each).  GELU's normal distribution is Abramowitz and
+// Stegun 7.1.26 (|error of erf| <= 1.5e-7), a polynomial times exp(-g^2/2),
+// the exponential its slope needs too.  Both errors, and the flush of values
+// below 2^-126 to zero, lie far below the 16-bit rounding of the result.
 __device__ __forceinline__ void activation(int act, float g, float& value, float& slope) {
   if (act == CCV_ACTIVATION_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    const float s = rcp(1.f + ex2(g * -1.4426950408889634f));
     value = g * s;
-    slope = s * (1.f + g * (1.f - s));
+    slope = fmaf(-value, s, value) + s;
   } else {
-    const float x = fabsf(g) * 0.70710678118654752f;
-    const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float e = __expf(-x * x);
+    const float t = rcp(fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.f));
+    const float e = ex2(g * g * (-0.5f * 1.4426950408889634f));
     float q = fmaf(t, 1.061405429f, -1.453152027f);
     q = fmaf(t, q, 1.421413741f);
     q = fmaf(t, q, -0.284496736f);
@@ -204,8 +233,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
   // full[S] (even CTA), empty[S], tfull[2], tempty[2] (even CTA), done,
-  // loaded[8] (GRAD: an epilogue warp's g and u), the TMEM address, flags.
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 5 + kEpiWarps);
+  // loaded[2][8] (GRAD: an epilogue warp's g and u), the TMEM address, flags.
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 5 + 2 * kEpiWarps);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_holder + 1);  // [0] skip, [1] abort
 
   const int warp = threadIdx.x >> 5;
@@ -234,7 +263,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ptx::mbar_init(tempty_bar(b), 2 * kEpiWarps);  // both CTAs' epilogue warps
     }
     ptx::mbar_init(done_bar, 1);
-    for (int i = 0; i < kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
     ptx::fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -362,12 +391,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int half = e >> 2;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t staging = smem_base + C::kStagingOffset + e * kSlotBytes;
-    const uint32_t loaded = loaded_bar0 + 8u * e;
+    const uint32_t loaded = loaded_bar0 + 16u * e;
     const uint32_t tempty0 = ptx::mapa_shared(tempty_bar(0), 0);
     const uint32_t tempty1 = ptx::mapa_shared(tempty_bar(1), 0);
     Ring<2048> ring2{staging};
     Ring<4096> ring4{staging};
-    uint32_t loads = 0;
+    uint32_t loads = 0, loads_issued = 0;
     int i = 0;
     for (int u = cid; u < p.units && !skip; u += ncl, ++i) {
       const Unit w = decode(p, u);
@@ -377,18 +406,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row0 = (2 * w.tm + static_cast<int>(rank)) * kRows + quarter * 32;
       const bool rows_in = row0 < t.m;
       const uint32_t acc = t_row + static_cast<uint32_t>(buf * BN);
-      constexpr int kGradChunks = BN / 2 / 64;
-      // GRAD: g and u of this warp's first 64 columns arrive during the mainloop.
-      auto load_inputs = [&](int col) {
-        if (lane == 0) {
-          ptx::bulk_wait_read_all();
-          ptx::mbar_arrive_expect_tx(loaded, 8192);
-          ptx::tma_load_2d(staging, &p.in[0], loaded, col, row0);
-          ptx::tma_load_2d(staging + 4096, &p.in[1], loaded, col, row0);
-        }
-      };
+      // GRAD: g and u of 32 columns at a time, loaded a chunk ahead into two
+      // alternating slots (the first during the mainloop); results replace
+      // them there and are stored from there.
+      constexpr int kGradChunks = BN / 2 / 32;
       const int grad_col = w.tn * BN + half * (BN / 2);
-      if constexpr (MODE == GRAD) load_inputs(grad_col);
+      auto load_inputs = [&](int c) {
+        if (lane == 0) {
+          ptx::bulk_wait_read_all();  // the slot's last results have been read
+          const uint32_t slot = staging + (loads_issued & 1u) * 4096;
+          const uint32_t bar = loaded + 8u * (loads_issued & 1u);
+          ptx::mbar_arrive_expect_tx(bar, 4096);
+          ptx::tma_load_2d(slot, &p.in[0], bar, grad_col + 32 * c, row0);
+          ptx::tma_load_2d(slot + 2048, &p.in[1], bar, grad_col + 32 * c, row0);
+        }
+        ++loads_issued;
+      };
+      if constexpr (MODE == GRAD) load_inputs(0);
       bool ok = ptx::mbar_wait_bounded_backoff(tfull_bar(buf), use & 1u, p.status, kTimeoutCode);
       ptx::tc_fence_after();
       if (!ok) flags[1] = 1;
@@ -436,58 +470,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else if constexpr (MODE == GRAD) {
 #pragma unroll 1
         for (int c = 0; c < kGradChunks; ++c) {
-          const int col = grad_col + c * 64;
-          ok = ptx::mbar_wait_bounded_backoff(loaded, loads & 1u, p.status, kTimeoutCode) && ok;
+          if (c + 1 < kGradChunks) load_inputs(c + 1);
+          const int col = grad_col + c * 32;
+          const uint32_t slot = staging + (loads & 1u) * 4096;
+          uint32_t d[32];
+          ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 32, d);
+          ok = ptx::mbar_wait_bounded_backoff(loaded + 8u * (loads & 1u), (loads >> 1) & 1u,
+                                              p.status, kTimeoutCode) && ok;
           ++loads;
           if (!ok) flags[1] = 1;
-#pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            uint32_t d[32];
-            ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 64 + h * 32, d);
-            ptx::tmem_wait_ld();
-            ptx::reg_fence(d);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(d);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t ag = slot128(staging, lane, h * 4 + j);
-              const uint32_t au = slot128(staging + 4096, lane, h * 4 + j);
-              const uint4 g4 = ld_shared_v4(ag), u4 = ld_shared_v4(au);
-              const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
-              uint32_t og[4], ou[4];
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t ag = slot64(slot, lane, j);
+            const uint32_t au = slot64(slot + 2048, lane, j);
+            const uint4 g4 = ld_shared_v4(ag), u4 = ld_shared_v4(au);
+            const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+            uint32_t og[4], ou[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 gg = unpack2(gw[k], T()), uu = unpack2(uw[k], T());
-                const float d0 = __uint_as_float(d[8 * j + 2 * k]);
-                const float d1 = __uint_as_float(d[8 * j + 2 * k + 1]);
-                float v0, s0, v1, s1;
-                activation(p.act, gg.x, v0, s0);
-                activation(p.act, gg.y, v1, s1);
-                og[k] = pack2(d0 * uu.x * s0, d1 * uu.y * s1, T());
-                ou[k] = pack2(d0 * v0, d1 * v1, T());
-              }
-              // The results take the place of the inputs they came from.
-              st_shared_v4(ag, og[0], og[1], og[2], og[3]);
-              st_shared_v4(au, ou[0], ou[1], ou[2], ou[3]);
+            for (int k = 0; k < 4; ++k) {
+              const float2 gg = unpack2(gw[k], T()), uu = unpack2(uw[k], T());
+              const float d0 = __uint_as_float(d[8 * j + 2 * k]);
+              const float d1 = __uint_as_float(d[8 * j + 2 * k + 1]);
+              float v0, s0, v1, s1;
+              activation(p.act, gg.x, v0, s0);
+              activation(p.act, gg.y, v1, s1);
+              og[k] = pack2(d0 * uu.x * s0, d1 * uu.y * s1, T());
+              ou[k] = pack2(d0 * v0, d1 * v1, T());
             }
+            st_shared_v4(ag, og[0], og[1], og[2], og[3]);
+            st_shared_v4(au, ou[0], ou[1], ou[2], ou[3]);
           }
           publish();
           if (lane == 0) {
             if (ok && !flags[1] && rows_in && col < t.n) {
-              ptx::tma_store_2d(&p.out[0], staging, col, row0);
-              ptx::tma_store_2d(&p.out[1], staging + 4096, col, row0);
+              ptx::tma_store_2d(&p.out[0], slot, col, row0);
+              ptx::tma_store_2d(&p.out[1], slot + 2048, col, row0);
             }
             ptx::bulk_commit_group();
           }
-          if (c + 1 < kGradChunks) load_inputs(col + 64);
         }
-      } else if (p.splits > 1) {
-        // fp32 partial sums, 32 columns at a time: [problem][split][m][n].
+      } else if (w.part >= 0) {
+        // fp32 partial sums, 32 columns at a time.
 #pragma unroll 1
         for (int c = 0; c < BN / 2; c += 32) {
           uint32_t d[32];
           ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c, d);
           ptx::tmem_wait_ld();
           ptx::reg_fence(d);
-          const int col = w.tn * BN + half * (BN / 2) + c;
           const uint32_t slot = ring4.take(lane);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -495,8 +526,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           publish();
           if (lane == 0) {
-            if (store && rows_in && col < t.n) {
-              ptx::tma_store_3d(&p.out[w.problem], slot, col, row0, w.split);
+            if (store && rows_in) {
+              ptx::tma_store_3d(&p.partial, slot, half * (BN / 2) + c,
+                                static_cast<int>(rank) * kRows + quarter * 32, w.part);
             }
             ptx::bulk_commit_group();
           }
