@@ -363,9 +363,19 @@ int encode_tiled_typed(CUtensorMap* map, CUtensorMapDataType type, const void* b
   const CUtensorMapSwizzle sw = swizzle == kSwizzle128   ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : swizzle == kSwizzleNone ? CU_TENSOR_MAP_SWIZZLE_NONE
                                                           : CU_TENSOR_MAP_SWIZZLE_64B;
-  const CUresult r = g_encode_tiled(
-      map, type, rank, const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return g_encode_tiled(map, type, rank, const_cast<void*>(base), d, st, bx, es,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // This driver call needs a current context, which a host thread gets only
+    // with its first runtime call that works on the device (an autograd
+    // thread may not have made one).
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     return set_error(CCV_ERR_UNSUPPORTED,
                      "cuTensorMapEncodeTiled rejected the problem (error " + std::to_string(r) + ")");

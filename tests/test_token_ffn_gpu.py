@@ -160,6 +160,21 @@ def test_same_result_every_time_and_on_another_stream(rows, features, hidden):
     assert all(torch.equal(a, b) for a, b in zip(first, second))
 
 
+def test_first_cuda_work_of_a_host_thread():
+    """A thread that has made no CUDA call yet (its memory comes from the
+    caching allocator) can run the block."""
+    import threading
+    args = _inputs(100, 128, 256)[:4]
+    want = cc.gated_feed_forward(*args)
+    torch.cuda.synchronize()
+    got = []
+    t = threading.Thread(target=lambda: got.append(cc.gated_feed_forward(*args)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and torch.equal(got[0], want)
+
+
 def test_refusals():
     x, wg, wu, wd, dy = _inputs(4, 16, 24)
     with pytest.raises(TypeError, match="bfloat16 or float16"):
