@@ -34,6 +34,29 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint2 k) {
 
 constexpr int kUnroll = 4;
 constexpr int kDropoutThreads = 256;
+constexpr int kDropoutBlock = 8 * kDropoutThreads * kUnroll;  // elements of a block
+
+// Eight elements of group g: limit = threshold << 16, so a word's high part
+// passes when the word does, its low part when the word shifted up does.
+template <typename Tx, typename Tr, bool RESIDUAL>
+__device__ __forceinline__ void drop8(const Vec<Tx, 8>& x, const Vec<Tr, 8>& residual, int64_t g,
+                                      uint64_t offset, uint2 key, uint32_t limit, float scale,
+                                      float (&o)[8]) {
+  const uint4 r = philox4x32_10(
+      make_uint4(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32),
+                 static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
+      key);
+  const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    o[2 * j] = (word[j] << 16) >= limit ? to_f32(x.e[2 * j]) : 0.f;
+    o[2 * j + 1] = word[j] >= limit ? to_f32(x.e[2 * j + 1]) : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    o[j] = RESIDUAL ? fmaf(o[j], scale, to_f32(residual.e[j])) : o[j] * scale;
+  }
+}
 
 // A thread takes kUnroll groups of eight elements, a block's width apart:
 // the loads of all of them are in flight while their counters are hashed.
@@ -41,56 +64,51 @@ constexpr int kDropoutThreads = 256;
 template <typename Tx, typename Tr, bool RESIDUAL, bool VEC>
 __global__ void __launch_bounds__(kDropoutThreads)
     dropout_groups(const Tx* __restrict__ x, const Tr* __restrict__ residual, Tr* __restrict__ y,
-                   int64_t count, uint32_t threshold, float scale, uint64_t seed, uint64_t offset,
+                   int64_t count, uint32_t limit, float scale, uint64_t seed, uint64_t offset,
                    const int64_t* __restrict__ offset_dev) {
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   if (offset_dev != nullptr) offset = static_cast<uint64_t>(*offset_dev);
   const uint2 key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
-  const int64_t first =
-      static_cast<int64_t>(blockIdx.x) * (kDropoutThreads * kUnroll) + threadIdx.x;
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * kDropoutBlock;
+  const int64_t first = start / 8 + threadIdx.x;
+  x += start + threadIdx.x * 8;
+  y += start + threadIdx.x * 8;
+  if (RESIDUAL) residual += start + threadIdx.x * 8;
   Vec<Tx, 8> vx[kUnroll];
   Vec<Tr, 8> vr[kUnroll];
+  if (VEC && start + kDropoutBlock <= count) {
 #pragma unroll
-  for (int k = 0; k < kUnroll; ++k) {
-    const int64_t i = (first + k * kDropoutThreads) * 8;
-    if (VEC && i + 8 <= count) {
-      vx[k] = load_vec<Tx, 8>(x + i);
-      if (RESIDUAL) vr[k] = load_vec<Tr, 8>(residual + i);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (i + j < count) {
-          vx[k].e[j] = x[i + j];
-          if (RESIDUAL) vr[k].e[j] = residual[i + j];
-        }
-      }
+    for (int k = 0; k < kUnroll; ++k) {
+      vx[k] = load_vec<Tx, 8>(x + k * kDropoutThreads * 8);
+      if (RESIDUAL) vr[k] = load_vec<Tr, 8>(residual + k * kDropoutThreads * 8);
     }
-  }
 #pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      float o[8];
+      drop8<Tx, Tr, RESIDUAL>(vx[k], vr[k], first + k * kDropoutThreads, offset, key, limit, scale,
+                              o);
+      store_vec<Tr, 8>(y + k * kDropoutThreads * 8, o);
+    }
+    return;
+  }
+  // The last block, and views that no vector load fits.
+  const int64_t left = count - start - threadIdx.x * 8;
+#pragma unroll 1
   for (int k = 0; k < kUnroll; ++k) {
-    const int64_t g = first + k * kDropoutThreads;
-    const int64_t i = g * 8;
-    if (i >= count) break;
-    const uint4 r = philox4x32_10(
-        make_uint4(static_cast<uint32_t>(g), static_cast<uint32_t>(g >> 32),
-                   static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32)),
-        key);
-    const uint32_t word[4] = {r.x, r.y, r.z, r.w};
-    float o[8];
+    const int at = k * kDropoutThreads * 8;
+    if (at >= left) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t part = (j & 1) != 0 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu;
-      o[j] = part >= threshold ? to_f32(vx[k].e[j]) * scale : 0.f;
-      if (RESIDUAL) o[j] += to_f32(vr[k].e[j]);
+      const bool in = at + j < left;
+      vx[0].e[j] = in ? x[at + j] : from_f32<Tx>(0.f);
+      if (RESIDUAL) vr[0].e[j] = in ? residual[at + j] : from_f32<Tr>(0.f);
     }
-    if (VEC && i + 8 <= count) {
-      store_vec<Tr, 8>(y + i, o);
-    } else {
+    float o[8];
+    drop8<Tx, Tr, RESIDUAL>(vx[0], vr[0], first + k * kDropoutThreads, offset, key, limit, scale, o);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (i + j < count) y[i + j] = from_f32<Tr>(o[j]);
-      }
+    for (int j = 0; j < 8; ++j) {
+      if (at + j < left) y[at + j] = from_f32<Tr>(o[j]);
     }
   }
 }
@@ -98,15 +116,20 @@ __global__ void __launch_bounds__(kDropoutThreads)
 template <typename Tx, typename Tr, bool RESIDUAL, bool VEC>
 int launch_groups(const Dropout& a, cudaStream_t stream) {
   const uint32_t threshold = static_cast<uint32_t>(std::floor(a.p * 65536.0 + 0.5));
-  const float scale =
-      threshold >= 65536u ? 0.f : static_cast<float>(65536.0 / (65536.0 - threshold));
-  constexpr int64_t per_block = 8LL * kDropoutThreads * kUnroll;
-  const int64_t blocks = (a.count + per_block - 1) / per_block;
+  if (threshold == 65536u) {
+    // Everything is dropped: zeros, or the residual.
+    const size_t bytes = static_cast<size_t>(a.count) * sizeof(Tr);
+    if (!RESIDUAL) return launched(cudaMemsetAsync(a.y, 0, bytes, stream), "dropout");
+    return launched(cudaMemcpyAsync(a.y, a.residual, bytes, cudaMemcpyDeviceToDevice, stream),
+                    "dropout");
+  }
+  const float scale = static_cast<float>(65536.0 / (65536.0 - threshold));
+  const int64_t blocks = (a.count + kDropoutBlock - 1) / kDropoutBlock;
   return launched(
       launch_kernel(dropout_groups<Tx, Tr, RESIDUAL, VEC>, dim3(static_cast<unsigned>(blocks)),
                     dim3(kDropoutThreads), 0, stream, 1, static_cast<const Tx*>(a.x),
-                    static_cast<const Tr*>(a.residual), static_cast<Tr*>(a.y), a.count, threshold,
-                    scale, a.seed, a.offset, a.offset_dev),
+                    static_cast<const Tr*>(a.residual), static_cast<Tr*>(a.y), a.count,
+                    threshold << 16, scale, a.seed, a.offset, a.offset_dev),
       "dropout");
 }
 

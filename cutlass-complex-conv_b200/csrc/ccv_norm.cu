@@ -7,16 +7,26 @@
 //   dw_j = sum_rows dy_j z_j,   db_j = sum_rows dy_j
 //
 // Both directions are bound by memory: the forward pass reads x and writes y
-// once, the backward pass reads x and dy and writes dx once.  A group of G
-// threads holds a row in registers, so the mean, the centred squares and the
-// output come from one read; G is the fewest threads (a power of two within
-// a warp, then whole warps) that hold the row at 16 or 32 elements each, so
-// narrow rows share a warp and few shuffles are spent per element.  The
-// backward pass keeps each thread's columns fixed and sums dw and db over the
-// rows in registers, reading nothing twice; blocks leave fp32 partial sums
-// that a second launch adds in block order (deterministic).  Rows too wide
-// for a block's registers take kernels that read them again from the caches.
+// once, the backward pass reads x and dy and writes dx once.  One block of up
+// to 512 threads per SM walks the rows; a group of G threads holds a row, 16
+// elements each (G a power of two within a warp, then whole warps: narrow
+// rows share a warp and cost few shuffles per element).  Every thread copies
+// the vectors it will use itself into a shared-memory ring some rows ahead
+// (cp.async), so 64 KB and more per SM are in flight at all times and no
+// barrier guards the ring.  Its columns stay the same from row to row: the
+// weights are in registers, and the backward pass sums dw and db over the
+// rows there, reading nothing twice; blocks leave fp32 partial sums that a
+// second launch adds in block order (deterministic).
+//
+// Dense rows whose width no vector divides start at any element of a vector.
+// A group's rows are then a multiple of V rows apart, so they all start at
+// the same one, and the group's vectors are shifted by it: loads stay whole
+// aligned vectors, whose first and last elements may belong to the row's
+// neighbours and are ignored (SHIFT).  Other layouts take single elements,
+// and rows wider than 8192 the kernels further down.
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "ccv_internal.h"
 #include "ccv_ptx.cuh"
@@ -26,10 +36,434 @@ namespace ccv {
 
 namespace {
 
-// Sum over the G threads of a row's group: shuffles within a warp, then
-// (G > 32: the group is the block) one exchange through shared memory, in
-// warp order.  `red` holds 32 entries per call in flight; successive calls
-// alternate between two of them.
+constexpr int kHeld = 16;        // elements of a row per thread
+constexpr int kThreads = 512;    // most threads of a block
+constexpr int kRingBytes = 196 * 1024;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Sums over the G threads of a group: shuffles within a warp, then (G > 32)
+// an exchange through shared memory, added in warp order.  Successive calls
+// alternate between the halves of `red` [2][warps of the block][N].
+template <int N>
+struct GroupSum {
+  int g, group;
+  float* red;
+  int parity = 0;
+
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      if (o < g) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      }
+    }
+    if (g <= 32) return;
+    float* mine = red + parity * (kThreads / 32) * N;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine[(threadIdx.x >> 5) * N + i] = v[i];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(g) : "memory");
+    const int warps = g >> 5;
+    const float* first = mine + group * warps * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+    for (int w = 0; w < warps; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += first[w * N + i];
+    }
+    parity ^= 1;
+  }
+};
+
+// A thread's vectors of one tensor in one ring stage: 16 elements in VPT
+// vectors of V, each in pieces of up to 16 bytes.
+template <typename T, int V>
+struct Held {
+  static constexpr int kVpt = kHeld / V;
+  static constexpr int kPiece = V * sizeof(T) < 16 ? V * sizeof(T) : 16;
+  static constexpr int kPieces = V * sizeof(T) / kPiece;
+  static constexpr int kBytes = kHeld * sizeof(T);  // per thread
+  static __device__ __forceinline__ uint32_t address(uint32_t stage, int i, int q) {
+    return stage + ((i * kPieces + q) * blockDim.x + threadIdx.x) * kPiece;
+  }
+  static __device__ __forceinline__ void zero(uint32_t stage, int i) {
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) {
+      const uint32_t at = address(stage, i, q);
+      if constexpr (kPiece == 16) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+      } else if constexpr (kPiece == 8) {
+        asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at), "r"(0) : "memory");
+      }
+    }
+  }
+  // Vector i from column c of `row` on.
+  static __device__ __forceinline__ void fetch(uint32_t stage, int i, const T* row, int c) {
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) {
+      copy_async<kPiece>(address(stage, i, q), reinterpret_cast<const char*>(row + c) + q * kPiece);
+    }
+  }
+  // The same for a vector that reaches past the tensor's end.
+  static __device__ __forceinline__ void fetch_end(uint32_t stage, int i, const T* row, int c,
+                                                   int features) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (c + j < features) {
+        const uint32_t to =
+            address(stage, i, j * sizeof(T) / kPiece) + (j * sizeof(T)) % kPiece;
+        if constexpr (sizeof(T) == 4) {
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(to),
+                       "r"(*reinterpret_cast<const uint32_t*>(row + c + j))
+                       : "memory");
+        } else {
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(to),
+                       "h"(*reinterpret_cast<const uint16_t*>(row + c + j))
+                       : "memory");
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ Vec<T, V> read(const uint8_t* stage, int i) {
+    Vec<T, V> v;
+    using Piece = std::conditional_t<kPiece == 16, uint4, std::conditional_t<kPiece == 8, uint2,
+                  std::conditional_t<kPiece == 4, uint32_t, uint16_t>>>;
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) {
+      reinterpret_cast<Piece*>(&v)[q] = *reinterpret_cast<const Piece*>(
+          stage + ((i * kPieces + q) * blockDim.x + threadIdx.x) * kPiece);
+    }
+    return v;
+  }
+};
+
+// Zeroes the elements of a vector at column c that lie outside the row.
+template <typename T, int V>
+__device__ __forceinline__ void clip(Vec<T, V>& v, int c, int features) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (c + j < 0 || c + j >= features) v.e[j] = from_f32<T>(0.f);
+  }
+}
+
+// Ring stages for `bytes` per thread and row.
+template <int BYTES>
+constexpr int kRingStages =
+    kRingBytes / (kThreads * BYTES) < 6 ? kRingBytes / (kThreads * BYTES) : 6;
+
+// Forward, rows of up to 8192 features.
+template <typename Tx, typename Tw, typename Ty, int V, bool SHIFT>
+__global__ void __launch_bounds__(kThreads, 1)
+    norm_forward_ring(const Tx* __restrict__ x, int64_t x_stride, const Tw* __restrict__ w,
+                      const Tw* __restrict__ b, float eps, Ty* __restrict__ y,
+                      float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows,
+                      int features, int g) {
+  using Hx = Held<Tx, V>;
+  constexpr int VPT = Hx::kVpt;
+  constexpr int S = kRingStages<Hx::kBytes>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[2 * (kThreads / 32)];
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const int group = threadIdx.x / g;
+  const int lane = threadIdx.x - group * g;
+  const int per_block = blockDim.x / g;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  const int shift = SHIFT ? static_cast<int>((first + group) * features % V) : 0;
+  auto column = [&](int i) { return (i * g + lane) * V - shift; };
+  const uint32_t ring_base = ptx::smem_u32(ring);
+  const uint32_t stage_bytes = blockDim.x * Hx::kBytes;
+  auto fetch = [&](int stage, int64_t r) {
+    if (r < rows) {
+      const Tx* row = x + r * x_stride;
+      const uint32_t at = ring_base + stage * stage_bytes;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = column(i);
+        if (SHIFT && r == rows - 1 && c + V > features) {
+          Hx::fetch_end(at, i, row, c, features);
+        } else if (c < features) {
+          Hx::fetch(at, i, row, c);
+        }
+      }
+    }
+    copy_commit();
+  };
+  // Vectors past the row's end stay zero.
+  for (int k = 0; k < S; ++k) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (column(i) + V > features) Hx::zero(ring_base + k * stage_bytes, i);
+    }
+    fetch(k, first + group + k * step);
+  }
+  float wt[VPT][V], bs[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = column(i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool in = c + j >= 0 && c + j < features;
+      wt[i][j] = in && w != nullptr ? to_f32(w[c + j]) : 1.f;
+      bs[i][j] = in && b != nullptr ? to_f32(b[c + j]) : 0.f;
+    }
+  }
+  GroupSum<1> total{g, group, red};
+  const float n = static_cast<float>(features), inv = 1.f / n;
+  int stage = 0;
+  // The block's groups walk together: every thread takes part in each sum.
+  for (int64_t r0 = first; r0 < rows; r0 += step) {
+    const int64_t r = r0 + group;
+    const bool live = r < rows;
+    copy_wait<S - 1>();
+    float v[VPT][V];
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      Vec<Tx, V> q = Hx::read(ring + stage * stage_bytes, i);
+      const int c = column(i);
+      if (SHIFT && (c < 0 || c + V > features)) clip(q, c, features);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = to_f32(q.e[j]);
+        sum[0] += v[i][j];
+      }
+    }
+    fetch(stage, r + S * step);
+    stage = stage + 1 == S ? 0 : stage + 1;
+    total(sum);
+    const float mean = sum[0] / n;
+    float sq[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column(i);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] -= mean;
+      if (SHIFT && (c < 0 || c + V > features)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (c + j >= 0 && c + j < features) sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+        }
+      } else if (c < features) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+      }
+    }
+    total(sq);
+    const float rstd = rsqrtf(sq[0] * inv + eps);
+    if (!live) continue;
+    Ty* yr = y + r * features;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column(i);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = fmaf(v[i][j] * rstd, wt[i][j], bs[i][j]);
+      if (!SHIFT || (c >= 0 && c + V <= features)) {
+        if (c < features) store_vec<Ty, V>(yr + c, o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (c + j >= 0 && c + j < features) yr[c + j] = from_f32<Ty>(o[j]);
+        }
+      }
+    }
+    if (lane == 0) {
+      if (mean_out != nullptr) mean_out[r] = mean;
+      if (rstd_out != nullptr) rstd_out[r] = rstd;
+    }
+  }
+}
+
+// Backward, rows of up to 8192 features; partial: [blocks][2][features].
+// V = 1: single elements straight from global memory.
+template <typename Tx, typename Tw, typename Ty, int V, bool SHIFT>
+__global__ void __launch_bounds__(kThreads, 1)
+    norm_backward_ring(const Ty* __restrict__ dy, int64_t dy_stride, const Tx* __restrict__ x,
+                       int64_t x_stride, const float* __restrict__ mean_in,
+                       const float* __restrict__ rstd_in, const Tw* __restrict__ w,
+                       Tx* __restrict__ dx, float* __restrict__ partial, int64_t rows,
+                       int features, int g) {
+  using Hx = Held<Tx, V>;
+  using Hy = Held<Ty, V>;
+  constexpr int VPT = Hx::kVpt;
+  constexpr int S = kRingStages<Hx::kBytes + Hy::kBytes>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[2 * (kThreads / 32) * 2];
+  ptx::griddep_wait();
+  ptx::griddep_launch_dependents();
+  const int group = threadIdx.x / g;
+  const int lane = threadIdx.x - group * g;
+  const int per_block = blockDim.x / g;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  const int shift = SHIFT ? static_cast<int>((first + group) * features % V) : 0;
+  auto column = [&](int i) { return (i * g + lane) * V - shift; };
+  const uint32_t ring_base = ptx::smem_u32(ring);
+  const uint32_t x_bytes = blockDim.x * Hx::kBytes;
+  const uint32_t stage_bytes = x_bytes + blockDim.x * Hy::kBytes;
+  auto fetch = [&](int stage, int64_t r) {
+    if constexpr (V > 1) {
+      const uint32_t at = ring_base + stage * stage_bytes;
+      if (r < rows) {
+        const Tx* xr = x + r * x_stride;
+        const Ty* gr = dy + r * dy_stride;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = column(i);
+          if (SHIFT && r == rows - 1 && c + V > features) {
+            Hx::fetch_end(at, i, xr, c, features);
+            Hy::fetch_end(at + x_bytes, i, gr, c, features);
+          } else if (c < features) {
+            Hx::fetch(at, i, xr, c);
+            Hy::fetch(at + x_bytes, i, gr, c);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) Hy::zero(at + x_bytes, i);
+      }
+      copy_commit();
+    }
+  };
+  // Vectors past the row's end stay zero in dy, and rows past the last one
+  // become zero: they add nothing to any sum.  (x must only be finite there.)
+  if constexpr (V > 1) {
+    for (int k = 0; k < S; ++k) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (column(i) + V > features || first + group + k * step >= rows) {
+          Hx::zero(ring_base + k * stage_bytes, i);
+          Hy::zero(ring_base + k * stage_bytes + x_bytes, i);
+        }
+      }
+      fetch(k, first + group + k * step);
+    }
+  }
+  const float inv = 1.f / static_cast<float>(features);
+  float wt[VPT][V], dw[VPT][V] = {}, db[VPT][V] = {};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = column(i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      wt[i][j] = w != nullptr && c + j >= 0 && c + j < features ? to_f32(w[c + j]) : 1.f;
+    }
+  }
+  float mean = 0.f, rstd = 0.f;
+  if (first + group < rows) {
+    mean = mean_in[first + group];
+    rstd = rstd_in[first + group];
+  }
+  GroupSum<2> total{g, group, red};
+  int stage = 0;
+  // The block's groups walk together: every thread takes part in each sum.
+  for (int64_t r0 = first; r0 < rows; r0 += step) {
+    const int64_t r = r0 + group;
+    const bool live = r < rows;
+    const float scale = rstd;
+    if constexpr (V > 1) copy_wait<S - 1>();
+    float z[VPT][V], t[VPT][V];
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column(i);
+      Vec<Tx, V> qx;
+      Vec<Ty, V> qg;
+      if constexpr (V > 1) {
+        qx = Hx::read(ring + stage * stage_bytes, i);
+        qg = Hy::read(ring + stage * stage_bytes + x_bytes, i);
+        if (SHIFT && (c < 0 || c + V > features)) {
+          clip(qx, c, features);
+          clip(qg, c, features);
+        }
+      } else {
+        qx.e[0] = from_f32<Tx>(0.f);
+        qg.e[0] = from_f32<Ty>(0.f);
+        if (live && c < features) {
+          qx.e[0] = x[r * x_stride + c];
+          qg.e[0] = dy[r * dy_stride + c];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = to_f32(qg.e[j]);
+        z[i][j] = (to_f32(qx.e[j]) - mean) * scale;
+        t[i][j] = d * wt[i][j];
+        dw[i][j] = fmaf(d, z[i][j], dw[i][j]);
+        db[i][j] += d;
+        sum[0] += t[i][j];
+        sum[1] = fmaf(t[i][j], z[i][j], sum[1]);
+      }
+    }
+    fetch(stage, r + S * step);
+    stage = stage + 1 == S ? 0 : stage + 1;
+    if (r + step < rows) {
+      mean = mean_in[r + step];
+      rstd = rstd_in[r + step];
+    }
+    total(sum);
+    if (!live || dx == nullptr) continue;
+    const float a = sum[0] * inv, c1 = sum[1] * inv;
+    Tx* out = dx + r * features;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = column(i);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = scale * (t[i][j] - a - z[i][j] * c1);
+      if (!SHIFT || (c >= 0 && c + V <= features)) {
+        if (c < features) store_vec<Tx, V>(out + c, o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (c + j >= 0 && c + j < features) out[c + j] = from_f32<Tx>(o[j]);
+        }
+      }
+    }
+  }
+  // The groups' sums side by side in the ring's memory, then added in order.
+  copy_wait<0>();
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(ring);  // [groups][2][features]
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int c = column(i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (c + j >= 0 && c + j < features) {
+        sums[(group * 2) * features + c + j] = dw[i][j];
+        sums[(group * 2 + 1) * features + c + j] = db[i][j];
+      }
+    }
+  }
+  __syncthreads();
+  float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * features;
+  for (int c = threadIdx.x; c < 2 * features; c += blockDim.x) {
+    float v = 0.f;
+    for (int k = 0; k < per_block; ++k) v += sums[k * 2 * features + c];
+    out[c] = v;
+  }
+}
+
+// Sum over a row's G threads where the group is the block for G > 32.
 template <int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], int g, float (*red)[N]) {
 #pragma unroll
@@ -56,7 +490,8 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int g, float (*red)[N])
   }
 }
 
-// Forward, rows in registers: VPT vectors of V elements per thread.
+// Forward without the ring, VPT vectors of V elements per thread, one row per
+// group and launch: rows of more than 8192 features, and single elements.
 template <typename Tx, typename Tw, typename Ty, int V, int VPT>
 __global__ void __launch_bounds__(1024, 1)
     norm_forward_held(const Tx* __restrict__ x, int64_t x_stride, const Tw* __restrict__ w,
@@ -127,143 +562,6 @@ __global__ void __launch_bounds__(1024, 1)
     if (mean_out != nullptr) mean_out[row] = mean;
     if (rstd_out != nullptr) rstd_out[row] = rstd;
   }
-}
-
-constexpr int kBackwardThreads = 512;  // most threads of a backward block
-constexpr int kBackwardHeld = 16;      // elements per thread
-
-// Backward, rows in registers; partial: [blocks][2][features].
-template <typename Tx, typename Tw, typename Ty, int V>
-__global__ void __launch_bounds__(kBackwardThreads, 1)
-    norm_backward_held(const Ty* __restrict__ dy, int64_t dy_stride, const Tx* __restrict__ x,
-                       int64_t x_stride, const float* __restrict__ mean_in,
-                       const float* __restrict__ rstd_in, const Tw* __restrict__ w,
-                       Tx* __restrict__ dx, float* __restrict__ partial, int64_t rows,
-                       int features, int g) {
-  constexpr int VPT = kBackwardHeld / V;
-  __shared__ float red[2][kBackwardThreads / 32][2];
-  extern __shared__ float columns[];  // [2][features], g <= 32
-  ptx::griddep_wait();
-  ptx::griddep_launch_dependents();
-  const bool wide = g > 32;
-  const int lane = wide ? threadIdx.x : threadIdx.x & (g - 1);
-  const int per_block = wide ? 1 : blockDim.x / g;
-  const int group = wide ? 0 : threadIdx.x / g;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  const float inv = 1.f / static_cast<float>(features);
-  float wt[VPT][V], dw[VPT][V] = {}, db[VPT][V] = {};
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int c = (i * g + lane) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) wt[i][j] = 1.f;
-    if (w != nullptr && c < features) {
-      const Vec<Tw, V> wv = load_vec<Tw, V>(w + c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) wt[i][j] = to_f32(wv.e[j]);
-    }
-  }
-  Vec<Tx, V> rx[VPT];
-  Vec<Ty, V> rg[VPT];
-  float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](int64_t r) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = (i * g + lane) * V;
-      if (c < features) {
-        rx[i] = load_vec<Tx, V>(x + r * x_stride + c);
-        rg[i] = load_vec<Ty, V>(dy + r * dy_stride + c);
-      }
-    }
-    mean = mean_in[r];
-    rstd = rstd_in[r];
-  };
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
-  if (first + group < rows) fetch(first + group);
-  int parity = 0;
-  // The block's groups walk together: every thread takes part in each sum.
-  for (int64_t r0 = first; r0 < rows; r0 += step, parity ^= 1) {
-    const int64_t r = r0 + group;
-    const bool live = r < rows;
-    float z[VPT][V], t[VPT][V];
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const bool in = live && (i * g + lane) * V < features;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        z[i][j] = 0.f;
-        t[i][j] = 0.f;
-        if (in) {
-          const float d = to_f32(rg[i].e[j]);
-          z[i][j] = (to_f32(rx[i].e[j]) - mean) * rstd;
-          t[i][j] = d * wt[i][j];
-          dw[i][j] = fmaf(d, z[i][j], dw[i][j]);
-          db[i][j] += d;
-          sum[0] += t[i][j];
-          sum[1] = fmaf(t[i][j], z[i][j], sum[1]);
-        }
-      }
-    }
-    const float scale = rstd;
-    // The next row's loads are in flight during this row's sums and stores.
-    if (r + step < rows) fetch(r + step);
-    group_sum<2>(sum, g, red[parity]);
-    if (live && dx != nullptr) {
-      const float a = sum[0] * inv, c1 = sum[1] * inv;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = (i * g + lane) * V;
-        if (c < features) {
-          float o[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = scale * (t[i][j] - a - z[i][j] * c1);
-          store_vec<Tx, V>(dx + r * features + c, o);
-        }
-      }
-    }
-  }
-  float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * features;
-  if (wide) {
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = (i * g + lane) * V;
-      if (c < features) {
-        store_vec<float, V>(out + c, dw[i]);
-        store_vec<float, V>(out + features + c, db[i]);
-      }
-    }
-    return;
-  }
-  // Groups that share a warp add up by shuffles, the warps in turn.
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      for (int o = 16; o >= g; o >>= 1) {
-        dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], o);
-        db[i][j] += __shfl_xor_sync(0xffffffffu, db[i][j], o);
-      }
-    }
-  }
-  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  for (int k = 0; k < warps; ++k) {
-    if (warp == k && (threadIdx.x & 31) < g) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = (i * g + lane) * V + j;
-          if (c < features) {
-            columns[c] = k == 0 ? dw[i][j] : columns[c] + dw[i][j];
-            columns[features + c] = k == 0 ? db[i][j] : columns[features + c] + db[i][j];
-          }
-        }
-      }
-    }
-    __syncthreads();
-  }
-  for (int c = threadIdx.x; c < 2 * features; c += blockDim.x) out[c] = columns[c];
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -374,22 +672,22 @@ __global__ void norm_backward_columns(const Ty* __restrict__ dy, int64_t dy_stri
 }
 
 // dweight and dbias from the blocks' partial sums [slices][2][features]: 32
-// columns per block, eight warps take every eighth slice, then add up in
-// warp order.
+// columns per block, each warp takes every 32nd slice (its few loads are in
+// flight together), then they add up in warp order.
 template <typename Tw>
-__global__ void __launch_bounds__(256) norm_backward_reduce(const float* __restrict__ partial,
-                                                            int slices, Tw* __restrict__ dw,
-                                                            Tw* __restrict__ db,
-                                                            int64_t features) {
-  __shared__ float sh[2][8][32];
+__global__ void __launch_bounds__(1024) norm_backward_reduce(const float* __restrict__ partial,
+                                                             int slices, Tw* __restrict__ dw,
+                                                             Tw* __restrict__ db,
+                                                             int64_t features) {
+  __shared__ float sh[2][32][33];
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sw = 0.f, sb = 0.f;
   if (j < features) {
-#pragma unroll 4
-    for (int s = warp; s < slices; s += 8) {
+#pragma unroll 8
+    for (int s = warp; s < slices; s += 32) {
       sw += partial[(static_cast<int64_t>(s) * 2) * features + j];
       sb += partial[(static_cast<int64_t>(s) * 2 + 1) * features + j];
     }
@@ -397,14 +695,18 @@ __global__ void __launch_bounds__(256) norm_backward_reduce(const float* __restr
   sh[0][warp][lane] = sw;
   sh[1][warp][lane] = sb;
   __syncthreads();
-  if (warp < 2 && j < features) {
-    Tw* out = warp == 0 ? dw : db;
-    if (out != nullptr) {
-      float v = 0.f;
+  // Warp w adds columns' warps: lane l of warp w holds warp l's sum of column w.
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+  if (col >= features) return;
+  float a = sh[0][lane][warp], b = sh[1][lane][warp];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v += sh[warp][k][lane];
-      out[j] = from_f32<Tw>(v);
-    }
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if (lane == 0) {
+    if (dw != nullptr) dw[col] = from_f32<Tw>(a);
+    if (db != nullptr) db[col] = from_f32<Tw>(b);
   }
 }
 
@@ -428,9 +730,31 @@ int group_size(int64_t features, int per, int most) {
   return g;
 }
 
-int64_t backward_blocks(int64_t rows) {
-  // Two blocks of up to 256 threads per SM (128 registers each).
-  return std::max<int64_t>(1, std::min<int64_t>(rows, 2 * device_sm_count()));
+// Grid of the ring kernels.
+struct Rings {
+  int g, per_block, blocks;
+};
+
+// Groups of g threads; v > 1: a group's rows start at the same element of a
+// vector of v, so they are a multiple of v rows apart.
+Rings plan_rings(int64_t rows, int g, int v) {
+  const int sms = device_sm_count();
+  Rings p;
+  p.g = g;
+  p.per_block = static_cast<int>(
+      std::min<int64_t>(kThreads / g, std::max<int64_t>(1, (rows + sms - 1) / sms)));
+  if (g < 32) p.per_block = (p.per_block + 32 / g - 1) / (32 / g) * (32 / g);  // whole warps
+  const int64_t need = std::max<int64_t>(1, (rows + p.per_block - 1) / p.per_block);
+  int most = sms;
+  while (most > 1 && need > most && (static_cast<int64_t>(most) * p.per_block) % v != 0) --most;
+  p.blocks = static_cast<int>(std::min<int64_t>(need, most));
+  return p;
+}
+
+// Whether rows of `n` dense elements can be read as shifted vectors of V.
+template <typename T, int V>
+bool shifted_rows(const void* p, int64_t stride, int64_t n) {
+  return stride == n && vec_rows<T, V>(p, 0, V);
 }
 
 unsigned row_blocks(int64_t rows) {
@@ -455,27 +779,59 @@ int forward_held(const NormForward& a, int g, cudaStream_t stream) {
 template <typename Tx>
 constexpr int kWide = 16 / sizeof(Tx);
 
+template <auto KERNEL, typename... Args>
+int launch_ring(const Rings& p, size_t smem, cudaStream_t stream, const char* what, Args... args) {
+  static std::once_flag once[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaError_t e = cudaSuccess;
+  std::call_once(once[dev & 63], [&]() {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  });
+  if (e != cudaSuccess) return cuda_error(e, what);
+  return launched(launch_kernel(KERNEL, dim3(p.blocks), dim3(p.per_block * p.g), smem, stream, 1,
+                                args...),
+                  what);
+}
+
 template <typename Tx, typename Tw, typename Ty>
 struct RunForward {
-  template <int V>
+  static constexpr int V = kWide<Tx>;
+  template <bool SHIFT>
+  static int ring(const NormForward& a, cudaStream_t stream) {
+    const int g = group_size(a.features + (SHIFT ? V - 1 : 0), kHeld, kThreads);
+    const Rings p = plan_rings(a.rows, g, SHIFT ? V : 1);
+    const size_t smem =
+        static_cast<size_t>(p.per_block) * g * Held<Tx, V>::kBytes * kRingStages<Held<Tx, V>::kBytes>;
+    return launch_ring<norm_forward_ring<Tx, Tw, Ty, V, SHIFT>>(
+        p, smem, stream, "layer norm forward", static_cast<const Tx*>(a.x), a.x_stride,
+        static_cast<const Tw*>(a.weight), static_cast<const Tw*>(a.bias), a.eps,
+        static_cast<Ty*>(a.y), a.mean, a.rstd, a.rows, static_cast<int>(a.features), g);
+  }
+  template <int W>
   static int held(const NormForward& a, cudaStream_t stream) {
     // 32 elements per thread keep 513 to 1024 features within a warp (no
     // block-wide sum) and reach the widest rows.
     const int64_t d = a.features;
     if ((d > 512 && d <= 1024) || d > 16384) {
-      return forward_held<Tx, Tw, Ty, V, 32 / V>(a, group_size(d, 32, 1024), stream);
+      return forward_held<Tx, Tw, Ty, W, 32 / W>(a, group_size(d, 32, 1024), stream);
     }
-    return forward_held<Tx, Tw, Ty, V, 16 / V>(a, group_size(d, 16, 1024), stream);
+    return forward_held<Tx, Tw, Ty, W, 16 / W>(a, group_size(d, 16, 1024), stream);
   }
   static int run(const NormForward& a, cudaStream_t stream) {
-    constexpr int V = kWide<Tx>;
-    if (a.features <= 32768) {
-      if (vec_rows<Tx, V>(a.x, a.x_stride, a.features) &&
-          vec_rows<Ty, V>(a.y, a.features, a.features) &&
-          vec_rows<Tw, V>(a.weight, 0, a.features) && vec_rows<Tw, V>(a.bias, 0, a.features)) {
-        return held<V>(a, stream);
+    const bool wide = vec_rows<Tx, V>(a.x, a.x_stride, a.features) &&
+                      vec_rows<Ty, V>(a.y, a.features, a.features);
+    if (a.features <= kThreads * kHeld - V + 1) {
+      if (wide) return ring<false>(a, stream);
+      if (shifted_rows<Tx, V>(a.x, a.x_stride, a.features) &&
+          shifted_rows<Ty, V>(a.y, a.features, a.features)) {
+        return ring<true>(a, stream);
       }
-      return held<1>(a, stream);
+    }
+    if (a.features <= 32768) {
+      return wide && vec_rows<Tw, V>(a.weight, 0, V) && vec_rows<Tw, V>(a.bias, 0, V)
+                 ? held<V>(a, stream)
+                 : held<1>(a, stream);
     }
     return launched(
         launch_kernel(norm_forward_rows<Tx, Tw, Ty>, dim3(row_blocks(a.rows)), dim3(256), 0, stream,
@@ -488,35 +844,39 @@ struct RunForward {
 
 template <typename Tx, typename Tw, typename Ty>
 struct RunBackward {
-  template <int V>
-  static int held(const NormBackward& a, int g, int64_t blocks, float* partial,
-                  cudaStream_t stream) {
-    const size_t smem = g > 32 ? 0 : static_cast<size_t>(a.features) * 2 * sizeof(float);
-    return launched(
-        launch_kernel(norm_backward_held<Tx, Tw, Ty, V>, dim3(static_cast<unsigned>(blocks)),
-                      dim3(g > 32 ? g : 256), smem, stream, 1, static_cast<const Ty*>(a.dy),
-                      a.dy_stride, static_cast<const Tx*>(a.x), a.x_stride, a.mean, a.rstd,
-                      static_cast<const Tw*>(a.weight), static_cast<Tx*>(a.dx), partial, a.rows,
-                      static_cast<int>(a.features), g),
-        "layer norm backward");
+  static constexpr int V = kWide<Tx>;
+  template <int W, bool SHIFT>
+  static int ring(const NormBackward& a, float* partial, int* slices, cudaStream_t stream) {
+    constexpr int bytes = Held<Tx, W>::kBytes + Held<Ty, W>::kBytes;
+    const int g = group_size(a.features + (SHIFT ? W - 1 : 0), kHeld, kThreads);
+    const Rings p = plan_rings(a.rows, g, SHIFT ? W : 1);
+    *slices = p.blocks;
+    const size_t sums = static_cast<size_t>(p.per_block) * 2 * a.features * sizeof(float);
+    const size_t stages =
+        W > 1 ? static_cast<size_t>(p.per_block) * g * bytes * kRingStages<bytes> : 0;
+    return launch_ring<norm_backward_ring<Tx, Tw, Ty, W, SHIFT>>(
+        p, std::max(sums, stages), stream, "layer norm backward", static_cast<const Ty*>(a.dy),
+        a.dy_stride, static_cast<const Tx*>(a.x), a.x_stride, a.mean, a.rstd,
+        static_cast<const Tw*>(a.weight), static_cast<Tx*>(a.dx), partial, a.rows,
+        static_cast<int>(a.features), g);
   }
   static int run(const NormBackward& a, void* ws, cudaStream_t stream) {
-    constexpr int V = kWide<Tx>;
     float* partial = static_cast<float*>(ws);
     const Ty* dy = static_cast<const Ty*>(a.dy);
     const Tx* x = static_cast<const Tx*>(a.x);
-    const int g = group_size(a.features, kBackwardHeld, kBackwardThreads);
-    int slices;
+    const int64_t d = a.features;
+    int slices = 0;
     int rc = CCV_OK;
-    if (g > 0) {
-      const int64_t per_block = g > 32 ? 1 : 256 / g;
-      const int64_t blocks = backward_blocks((a.rows + per_block - 1) / per_block);
-      slices = static_cast<int>(blocks);
-      const bool wide = vec_rows<Tx, V>(x, a.x_stride, a.features) &&
-                        vec_rows<Ty, V>(dy, a.dy_stride, a.features) &&
-                        vec_rows<Tx, V>(a.dx, a.features, a.features) &&
-                        vec_rows<Tw, V>(a.weight, 0, a.features);
-      rc = wide ? held<V>(a, g, blocks, partial, stream) : held<1>(a, g, blocks, partial, stream);
+    if (d <= kThreads * kHeld - V + 1) {
+      if (vec_rows<Tx, V>(x, a.x_stride, d) && vec_rows<Ty, V>(dy, a.dy_stride, d) &&
+          vec_rows<Tx, V>(a.dx, d, d)) {
+        rc = ring<V, false>(a, partial, &slices, stream);
+      } else if (shifted_rows<Tx, V>(x, a.x_stride, d) && shifted_rows<Ty, V>(dy, a.dy_stride, d) &&
+                 shifted_rows<Tx, V>(a.dx, d, d)) {
+        rc = ring<V, true>(a, partial, &slices, stream);
+      } else {
+        rc = ring<1, false>(a, partial, &slices, stream);
+      }
     } else {
       slices = column_slices(a.rows);
       if (a.dx != nullptr && a.rows > 0) {
@@ -538,7 +898,7 @@ struct RunBackward {
     if (rc != CCV_OK || (a.dweight == nullptr && a.dbias == nullptr)) return rc;
     return launched(
         launch_kernel(norm_backward_reduce<Tw>,
-                      dim3(static_cast<unsigned>((a.features + 31) / 32)), dim3(256), 0, stream, 1,
+                      dim3(static_cast<unsigned>((a.features + 31) / 32)), dim3(1024), 0, stream, 1,
                       static_cast<const float*>(partial), slices, static_cast<Tw*>(a.dweight),
                       static_cast<Tw*>(a.dbias), a.features),
         "layer norm backward reduce");
@@ -569,9 +929,10 @@ int dispatch(int x_dtype, int weight_dtype, int y_dtype, Args&&... args) {
 }  // namespace
 
 size_t norm_backward_workspace_bytes(int64_t rows, int64_t features) {
-  const int64_t slices = group_size(features, kBackwardHeld, kBackwardThreads) > 0
-                             ? backward_blocks(rows)
-                             : column_slices(rows);
+  // Blocks of the ring kernels, or slices of the wide rows' column sums.
+  const int64_t slices =
+      std::max<int64_t>(std::min<int64_t>(std::max<int64_t>(rows, 1), device_sm_count()),
+                        column_slices(rows));
   return static_cast<size_t>(slices) * 2 * static_cast<size_t>(features) * sizeof(float);
 }
 
