@@ -115,6 +115,8 @@ Knobs parse_knobs() {
   k.streamk = env_int("CCV_STREAMK", -1);
   k.max_clusters = env_int("CCV_MAX_CLUSTERS", 0);
   k.tma_store = env_int("CCV_TMA_STORE", 1);
+  k.ffn_bn = env_int("CCV_FFN_BN", 0);
+  k.ffn_splits = env_int("CCV_FFN_SPLITS", 0);
   return k;
 }
 

@@ -218,6 +218,7 @@ Plan make_plan(const Extent* e, int problems, int64_t ksteps, bool may_split, bo
   Plan best;
   double best_cost = 1e30;
   for (int bn : {256, 128}) {
+    if (knobs().ffn_bn != 0 && knobs().ffn_bn != bn) continue;
     const int64_t tiles = tile_count(e, problems, gate ? bn / 2 : bn);
     const double step = bn == 256 ? 512.0 : 435.0;
     const int64_t full = tiles / clusters * clusters;
@@ -225,6 +226,7 @@ Plan make_plan(const Extent* e, int problems, int64_t ksteps, bool may_split, bo
     const double base = static_cast<double>(full / clusters) * ksteps * step;
     const int most = rest > 0 && may_split ? static_cast<int>(std::min<int64_t>(64, ksteps)) : 1;
     for (int splits = 1; splits <= most; ++splits) {
+      if (knobs().ffn_splits != 0 && splits != std::min(most, knobs().ffn_splits)) continue;
       double cost = base;
       if (rest > 0) {
         cost += static_cast<double>(ceil_div(rest * splits, clusters) * ceil_div(ksteps, splits)) *
@@ -278,7 +280,7 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
     err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (err != cudaSuccess) return;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * 148, 1, 1);
+    cfg.gridDim = dim3(4 * 148, 1, 1);
     cfg.blockDim = dim3(ffn::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     int n = 0;
@@ -286,7 +288,7 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
       max_clusters[dev & 63] = n;
     } else {
       cudaGetLastError();
-      max_clusters[dev & 63] = device_sm_count() / 2;
+      max_clusters[dev & 63] = device_sm_count() / 2 * C::kBlocksPerSm;
     }
   });
   if (err != cudaSuccess) return cuda_error(err, "cudaFuncSetAttribute(ffn)");

@@ -40,7 +40,6 @@ constexpr int kStepK = 64;        // reduction elements per pipeline stage: 128-
 constexpr int kOperandA = kRows * kStepK * 2;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kSlotBytes = 8192;  // staging of one epilogue warp
 constexpr int kMaxProblems = 3;
 constexpr int kRasterRows = 8;    // tile rows walked together (operand reuse in L2)
 constexpr int kTimeoutCode = CCV_ERR_DEVICE_TIMEOUT;
@@ -74,8 +73,13 @@ template <int MODE, int BN>
 struct Config {
   static constexpr int kOperandB = BN / 2 * kStepK * 2;
   static constexpr int kStage = kOperandA + kOperandB;
-  static constexpr int kStaging = kEpiWarps * kSlotBytes;
-  static constexpr int kStages = BN == 256 ? 5 : 6;
+  // BN = 256: one block per SM with five stages.  BN = 128, for problems of
+  // few tiles: three stages and half the staging, so that two blocks share an
+  // SM and the next launch's blocks start up beside this one's.
+  static constexpr int kBlocksPerSm = BN == 256 ? 1 : 2;
+  static constexpr int kWarpStaging = BN == 256 ? 8192 : 4096;
+  static constexpr int kStaging = kEpiWarps * kWarpStaging;
+  static constexpr int kStages = BN == 256 ? 5 : 3;
   static constexpr int kStagingOffset = kStages * kStage;
   static constexpr int kBarOffset = kStagingOffset + kStaging;
   static constexpr int kBarBytes = 512;
@@ -203,9 +207,9 @@ __device__ __forceinline__ uint32_t slot128(uint32_t slot, int row, int j) {
 
 // An epilogue warp's ring of staging slots of BYTES each, written by its
 // lanes and read by TMA stores.
-template <int BYTES>
+template <int TOTAL, int BYTES>
 struct Ring {
-  static constexpr int kSlots = kSlotBytes / BYTES;
+  static constexpr int kSlots = TOTAL / BYTES;
   uint32_t base;
   uint32_t next = 0;
   // A slot no store still reads.
@@ -225,7 +229,7 @@ __device__ __forceinline__ void publish() {
 }
 
 template <typename T, int MODE, int BN, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MODE, BN>::kBlocksPerSm)
     ffn_gemm_kernel(const __grid_constant__ GemmParams p) {
   using C = Config<MODE, BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -266,6 +270,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2 * kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
     ptx::fence_mbar_init();
   }
+  // A timeout reported by an earlier kernel: this one exits without work.
+  if (threadIdx.x == 32) flags[0] = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&p.a[0]);
     ptx::prefetch_tmap(&p.b[MODE == GATE ? rank : 0]);
@@ -281,8 +287,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   // Everything above may overlap the previous kernel on the stream.
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  if (threadIdx.x == 0) flags[0] = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
-  ptx::cta_sync();
   const uint32_t tmem_base = *tmem_holder;
   const bool skip = flags[0] != 0;
 
@@ -390,12 +394,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     const int half = e >> 2;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t staging = smem_base + C::kStagingOffset + e * kSlotBytes;
+    const uint32_t staging = smem_base + C::kStagingOffset + e * C::kWarpStaging;
     const uint32_t loaded = loaded_bar0 + 16u * e;
     const uint32_t tempty0 = ptx::mapa_shared(tempty_bar(0), 0);
     const uint32_t tempty1 = ptx::mapa_shared(tempty_bar(1), 0);
-    Ring<2048> ring2{staging};
-    Ring<4096> ring4{staging};
+    Ring<C::kWarpStaging, 2048> ring2{staging};
+    Ring<C::kWarpStaging, 4096> ring4{staging};
     uint32_t loads = 0, loads_issued = 0;
     int i = 0;
     for (int u = cid; u < p.units && !skip; u += ncl, ++i) {
@@ -406,16 +410,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row0 = (2 * w.tm + static_cast<int>(rank)) * kRows + quarter * 32;
       const bool rows_in = row0 < t.m;
       const uint32_t acc = t_row + static_cast<uint32_t>(buf * BN);
-      // GRAD: g and u of 32 columns at a time, loaded a chunk ahead into two
-      // alternating slots (the first during the mainloop); results replace
-      // them there and are stored from there.
+      // GRAD: g and u of 32 columns at a time, the first during the mainloop
+      // and (two slots) a chunk ahead; results replace them in their slot and
+      // are stored from there.
       constexpr int kGradChunks = BN / 2 / 32;
+      constexpr uint32_t kGradSlots = C::kWarpStaging / 4096;
       const int grad_col = w.tn * BN + half * (BN / 2);
       auto load_inputs = [&](int c) {
         if (lane == 0) {
           ptx::bulk_wait_read_all();  // the slot's last results have been read
-          const uint32_t slot = staging + (loads_issued & 1u) * 4096;
-          const uint32_t bar = loaded + 8u * (loads_issued & 1u);
+          const uint32_t slot = staging + (loads_issued % kGradSlots) * 4096;
+          const uint32_t bar = loaded + 8u * (loads_issued % kGradSlots);
           ptx::mbar_arrive_expect_tx(bar, 4096);
           ptx::tma_load_2d(slot, &p.in[0], bar, grad_col + 32 * c, row0);
           ptx::tma_load_2d(slot + 2048, &p.in[1], bar, grad_col + 32 * c, row0);
@@ -470,12 +475,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else if constexpr (MODE == GRAD) {
 #pragma unroll 1
         for (int c = 0; c < kGradChunks; ++c) {
-          if (c + 1 < kGradChunks) load_inputs(c + 1);
+          if (kGradSlots > 1 && c + 1 < kGradChunks) load_inputs(c + 1);
           const int col = grad_col + c * 32;
-          const uint32_t slot = staging + (loads & 1u) * 4096;
+          const uint32_t slot = staging + (loads % kGradSlots) * 4096;
           uint32_t d[32];
           ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 32, d);
-          ok = ptx::mbar_wait_bounded_backoff(loaded + 8u * (loads & 1u), (loads >> 1) & 1u,
+          ok = ptx::mbar_wait_bounded_backoff(loaded + 8u * (loads % kGradSlots), (loads / kGradSlots) & 1u,
                                               p.status, kTimeoutCode) && ok;
           ++loads;
           if (!ok) flags[1] = 1;
@@ -510,6 +515,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             ptx::bulk_commit_group();
           }
+          if (kGradSlots == 1 && c + 1 < kGradChunks) load_inputs(c + 1);
         }
       } else if (w.part >= 0) {
         // fp32 partial sums, 32 columns at a time.

@@ -50,6 +50,8 @@ struct Knobs {
   int streamk = -1;       // CCV_STREAMK=0|1: never / whenever possible (-1 model)
   int max_clusters = 0;   // CCV_MAX_CLUSTERS=n: persistent grid cap (0 none)
   int tma_store = 1;      // CCV_TMA_STORE=0: planar epilogue without TMA stores
+  int ffn_bn = 0;         // CCV_FFN_BN=128|256: feed-forward tile width (0 auto)
+  int ffn_splits = 0;     // CCV_FFN_SPLITS=n: parts of a feed-forward tail tile (0 auto)
 };
 const Knobs& knobs();
 void reload_knobs();
