@@ -245,7 +245,7 @@ std::tuple<torch::Tensor, torch::Tensor> gated_ffn_forward(torch::Tensor x, torc
   size_t saved_bytes = 0;
   if (save) {
     saved_bytes = ccv_gated_ffn_saved_bytes(r.rows, r.features, w.hidden);
-    saved = torch::empty({3, r.rows, saved_width(w.hidden)}, x.options());
+    saved = torch::empty({4, r.rows, saved_width(w.hidden)}, x.options());
   }
   const size_t bytes = ccv_gated_ffn_forward_workspace_bytes(r.rows, r.features, w.hidden, save);
   auto ws = scratch(bytes, x);
@@ -273,7 +273,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn
   check_like(saved, x, "saved");
   const Rows rx = as_tma_rows(x), rdy = as_tma_rows(dy);
   TORCH_CHECK_VALUE(saved.scalar_type() == x.scalar_type() && saved.is_contiguous() &&
-                        saved.dim() == 3 && saved.size(0) == 3 && saved.size(1) == rx.rows &&
+                        saved.dim() == 3 && saved.size(0) == 4 && saved.size(1) == rx.rows &&
                         saved.size(2) == saved_width(w.hidden),
                     "saved must be what the forward call returned for these shapes");
   torch::Tensor dx, dg, du, dd;

@@ -3,9 +3,10 @@
 //   g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g),
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
-// with x [M, D], Wg and Wu [F, D], Wd [D, F].  g, u, h, dg and du are rounded
-// to the operands' type once each: they are operands of the next product,
-// whose inputs the tensor cores take in 16 bits.
+// with x [M, D], Wg and Wu [F, D], Wd [D, F].  h, dg and du are rounded to the
+// operands' type once each: they are operands of the next product, whose
+// inputs the tensor cores take in 16 bits.  g and u are kept for the backward
+// pass to 24 bits.
 //
 // Forward: GATE, PLAIN.  Backward: GRAD, PLAIN over two segments (dx), PLAIN
 // over three problems in one launch (the weight gradients).  This file plans
@@ -121,7 +122,7 @@ constexpr int64_t kFewRows = 16;
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T, int NT>
-int launch_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t stream) {
+int launch_rows(const FfnForward& f, void* h, void* const (&planes)[3], cudaStream_t stream) {
   const FfnShape& s = f.shape;
   const int64_t sms = device_sm_count(), fp = padded(s.hidden);
   ffn::RowsParams p = {};
@@ -130,8 +131,9 @@ int launch_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t str
   p.w0 = static_cast<const uint16_t*>(f.w_gate);
   p.w1 = static_cast<const uint16_t*>(f.w_up);
   p.out = static_cast<uint16_t*>(h);
-  p.g = static_cast<uint16_t*>(g);
-  p.u = static_cast<uint16_t*>(u);
+  p.g = static_cast<uint16_t*>(planes[0]);
+  p.u = static_cast<uint16_t*>(planes[1]);
+  p.next = static_cast<uint16_t*>(planes[2]);
   p.out_stride = fp;
   p.rows = static_cast<int>(s.rows);
   p.k = static_cast<int>(s.features);
@@ -178,9 +180,9 @@ int launch_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t str
 }
 
 template <typename T>
-int run_rows(const FfnForward& f, void* h, void* g, void* u, cudaStream_t stream) {
-  return f.shape.rows <= 8 ? launch_rows<T, 1>(f, h, g, u, stream)
-                           : launch_rows<T, 2>(f, h, g, u, stream);
+int run_rows(const FfnForward& f, void* h, void* const (&planes)[3], cudaStream_t stream) {
+  return f.shape.rows <= 8 ? launch_rows<T, 1>(f, h, planes, stream)
+                           : launch_rows<T, 2>(f, h, planes, stream);
 }
 
 // ------------------------------------------------------------ planning
@@ -343,6 +345,10 @@ struct Product {
     sums.out[i] = base;
     sums.ldo[i] = ld;
   }
+  // A plane of 16-bit words read or written 32 columns at a time.
+  void plane(CUtensorMap* map, const void* base, int64_t m, int64_t n, int64_t ld) {
+    if (rc == CCV_OK) rc = encode_2d(map, dtype, base, n, m, ld, 32, 32);
+  }
   // Storage for the split tiles' parts (none without a split).
   void partials(void* base) {
     if (plan.tail == 0 || rc != CCV_OK) return;
@@ -499,10 +505,10 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   const ForwardPlan p = plan_forward(s, saved != nullptr, c);
   if (m <= kFewRows) {
     void* h = saved != nullptr ? saved : p.h;
-    void* g = saved != nullptr ? saved + plane : nullptr;
-    void* u = saved != nullptr ? saved + 2 * plane : nullptr;
-    return s.dtype == CCV_DTYPE_BF16 ? run_rows<__nv_bfloat16>(f, h, g, u, stream)
-                                     : run_rows<__half>(f, h, g, u, stream);
+    void* planes[3] = {};
+    for (int i = 0; i < 3 && saved != nullptr; ++i) planes[i] = saved + (i + 1) * plane;
+    return s.dtype == CCV_DTYPE_BF16 ? run_rows<__nv_bfloat16>(f, h, planes, stream)
+                                     : run_rows<__half>(f, h, planes, stream);
   }
   const Padded x{f.x, f.x_stride, m, d, p.x}, wg{f.w_gate, d, hid, d, p.w_gate},
       wu{f.w_up, d, hid, d, p.w_up}, wd{f.w_down, hid, d, hid, p.w_down};
@@ -518,8 +524,7 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
     g.operand_b(1, wu.matrix());
     g.result(0, h, m, hid, fp);
     if (saved != nullptr) {
-      g.result(1, saved + plane, m, hid, fp);
-      g.result(2, saved + 2 * plane, m, hid, fp);
+      for (int i = 1; i <= 3; ++i) g.plane(&g.prm.out[i], saved + i * plane, m, hid, fp);
       g.prm.save = 1;
     }
     g.problem(0, m, hid);
@@ -570,9 +575,7 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
     g.operand_b(0, wd.matrix());
     g.result(0, p.dg, m, hid, fp);
     g.result(1, p.du, m, hid, fp);
-    for (int i = 0; i < 2 && g.rc == CCV_OK; ++i) {
-      g.rc = encode_2d(&g.prm.in[i], s.dtype, saved + (i + 1) * plane, hid, m, fp, 32, 32);
-    }
+    for (int i = 0; i < 3; ++i) g.plane(&g.prm.in[i], saved + (i + 1) * plane, m, hid, fp);
     g.problem(0, m, hid);
     if ((rc = g.launch(stream)) != CCV_OK) return rc;
   }

@@ -54,8 +54,9 @@ struct alignas(64) GemmParams {
   // One problem: segments of the reduction, a[s] with b[s] (GATE: b[0] gate
   // rows, b[1] up rows).  Several problems: one segment each.
   CUtensorMap a[kMaxProblems], b[kMaxProblems];
-  CUtensorMap out[kMaxProblems];  // GATE: h, g, u; GRAD: dg, du; PLAIN: per problem
-  CUtensorMap in[2];              // GRAD: g, u
+  CUtensorMap out[4];  // GATE: h and (saving) the three planes of g and u; GRAD: dg, du;
+                       // PLAIN: per problem
+  CUtensorMap in[3];   // GRAD: the planes of g and u
   CUtensorMap partial;            // split tiles: fp32 [tile part][256][BN]
   Tiles tiles[kMaxProblems];
   int* status;
@@ -73,13 +74,14 @@ template <int MODE, int BN>
 struct Config {
   static constexpr int kOperandB = BN / 2 * kStepK * 2;
   static constexpr int kStage = kOperandA + kOperandB;
-  // BN = 256: one block per SM with five stages.  BN = 128, for problems of
-  // few tiles: three stages and half the staging, so that two blocks share an
-  // SM and the next launch's blocks start up beside this one's.
-  static constexpr int kBlocksPerSm = BN == 256 ? 1 : 2;
-  static constexpr int kWarpStaging = BN == 256 ? 8192 : 4096;
+  // BN = 256: one block per SM.  BN = 128, for problems of few tiles: few
+  // stages and little staging, so that two blocks share an SM and the next
+  // launch's blocks start up beside this one's.  GRAD trades a stage for room
+  // to load its inputs a chunk ahead.
+  static constexpr int kBlocksPerSm = BN == 256 || MODE == GRAD ? 1 : 2;
+  static constexpr int kWarpStaging = MODE == GRAD ? 12288 : (BN == 256 ? 8192 : 4096);
   static constexpr int kStaging = kEpiWarps * kWarpStaging;
-  static constexpr int kStages = BN == 256 ? 5 : 3;
+  static constexpr int kStages = MODE == GRAD ? (BN == 256 ? 4 : 5) : (BN == 256 ? 5 : 3);
   static constexpr int kStagingOffset = kStages * kStage;
   static constexpr int kBarOffset = kStagingOffset + kStaging;
   static constexpr int kBarBytes = 512;
@@ -174,11 +176,25 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float2 unpack2(uint32_t v, __nv_bfloat16) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+// g and u for the backward pass, to 24 bits of float32 each (a relative step
+// of 2^-15; 16 bits of either would show in dx and in the weight gradients
+// beside the roundings of dg and of the result): planes of the high 16 bits
+// of g, of u, and of the next 8 bits of both (g's in the low byte).
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __byte_perm(a, b, 0x7632);
 }
-__device__ __forceinline__ float2 unpack2(uint32_t v, __half) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+__device__ __forceinline__ uint32_t next_bytes(uint32_t g0, uint32_t u0, uint32_t g1, uint32_t u1) {
+  return __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
+}
+// The values of one plane word (two elements) and their word of next bytes;
+// the lowest byte repeats the next one, below the 24 bits.
+__device__ __forceinline__ float2 unpack_g(uint32_t high, uint32_t next) {
+  return make_float2(__uint_as_float(__byte_perm(high, next, 0x1044)),
+                     __uint_as_float(__byte_perm(high, next, 0x3266)));
+}
+__device__ __forceinline__ float2 unpack_u(uint32_t high, uint32_t next) {
+  return make_float2(__uint_as_float(__byte_perm(high, next, 0x1055)),
+                     __uint_as_float(__byte_perm(high, next, 0x3277)));
 }
 
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
@@ -410,20 +426,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
       const int row0 = (2 * w.tm + static_cast<int>(rank)) * kRows + quarter * 32;
       const bool rows_in = row0 < t.m;
       const uint32_t acc = t_row + static_cast<uint32_t>(buf * BN);
-      // GRAD: g and u of 32 columns at a time, the first during the mainloop
-      // and (two slots) a chunk ahead; results replace them in their slot and
-      // are stored from there.
+      // GRAD: the planes of g and u, 32 columns at a time, loaded a chunk ahead
+      // into two alternating slots (the first during the mainloop); dg and du
+      // replace the high halves there and are stored from there.
       constexpr int kGradChunks = BN / 2 / 32;
-      constexpr uint32_t kGradSlots = C::kWarpStaging / 4096;
+      constexpr uint32_t kGradBytes = 3 * 2048, kGradSlots = 2;
       const int grad_col = w.tn * BN + half * (BN / 2);
       auto load_inputs = [&](int c) {
         if (lane == 0) {
           ptx::bulk_wait_read_all();  // the slot's last results have been read
-          const uint32_t slot = staging + (loads_issued % kGradSlots) * 4096;
+          const uint32_t slot = staging + (loads_issued % kGradSlots) * kGradBytes;
           const uint32_t bar = loaded + 8u * (loads_issued % kGradSlots);
-          ptx::mbar_arrive_expect_tx(bar, 4096);
-          ptx::tma_load_2d(slot, &p.in[0], bar, grad_col + 32 * c, row0);
-          ptx::tma_load_2d(slot + 2048, &p.in[1], bar, grad_col + 32 * c, row0);
+          ptx::mbar_arrive_expect_tx(bar, kGradBytes);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            ptx::tma_load_2d(slot + 2048 * i, &p.in[i], bar, grad_col + 32 * c, row0);
+          }
         }
         ++loads_issued;
       };
@@ -445,16 +463,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           ptx::reg_fence(v);
           const int col = w.tn * (BN / 2) + fc;
           const bool in = store && rows_in && col < t.n;
-          auto put = [&](auto&& value, const CUtensorMap* map) {
+          // word(k): elements 2 k and 2 k + 1.
+          auto put = [&](auto&& word, const CUtensorMap* map) {
             const uint32_t slot = ring2.take(lane);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint32_t q[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                q[k] = pack2(value(8 * j + 2 * k), value(8 * j + 2 * k + 1), T());
-              }
-              st_shared_v4(slot64(slot, lane, j), q[0], q[1], q[2], q[3]);
+              st_shared_v4(slot64(slot, lane, j), word(4 * j), word(4 * j + 1), word(4 * j + 2),
+                           word(4 * j + 3));
             }
             publish();
             if (lane == 0) {
@@ -462,22 +477,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
               ptx::bulk_commit_group();
             }
           };
-          put([&](int j) {
-            float value, slope;
-            activation(p.act, __uint_as_float(g[j]), value, slope);
-            return value * __uint_as_float(v[j]);
+          put([&](int k) {
+            float v0, v1, slope;
+            activation(p.act, __uint_as_float(g[2 * k]), v0, slope);
+            activation(p.act, __uint_as_float(g[2 * k + 1]), v1, slope);
+            return pack2(v0 * __uint_as_float(v[2 * k]), v1 * __uint_as_float(v[2 * k + 1]), T());
           }, &p.out[0]);
           if (p.save) {
-            put([&](int j) { return __uint_as_float(g[j]); }, &p.out[1]);
-            put([&](int j) { return __uint_as_float(v[j]); }, &p.out[2]);
+            put([&](int k) { return high_halves(g[2 * k], g[2 * k + 1]); }, &p.out[1]);
+            put([&](int k) { return high_halves(v[2 * k], v[2 * k + 1]); }, &p.out[2]);
+            put([&](int k) { return next_bytes(g[2 * k], v[2 * k], g[2 * k + 1], v[2 * k + 1]); },
+                &p.out[3]);
           }
         }
       } else if constexpr (MODE == GRAD) {
 #pragma unroll 1
         for (int c = 0; c < kGradChunks; ++c) {
-          if (kGradSlots > 1 && c + 1 < kGradChunks) load_inputs(c + 1);
+          if (c + 1 < kGradChunks) load_inputs(c + 1);
           const int col = grad_col + c * 32;
-          const uint32_t slot = staging + (loads % kGradSlots) * 4096;
+          const uint32_t slot = staging + (loads % kGradSlots) * kGradBytes;
           uint32_t d[32];
           ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 32, d);
           ok = ptx::mbar_wait_bounded_backoff(loaded + 8u * (loads % kGradSlots), (loads / kGradSlots) & 1u,
@@ -491,11 +509,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
             const uint32_t ag = slot64(slot, lane, j);
             const uint32_t au = slot64(slot + 2048, lane, j);
             const uint4 g4 = ld_shared_v4(ag), u4 = ld_shared_v4(au);
+            const uint4 n4 = ld_shared_v4(slot64(slot + 4096, lane, j));
             const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, uw[4] = {u4.x, u4.y, u4.z, u4.w};
+            const uint32_t nw[4] = {n4.x, n4.y, n4.z, n4.w};
             uint32_t og[4], ou[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const float2 gg = unpack2(gw[k], T()), uu = unpack2(uw[k], T());
+              const float2 gg = unpack_g(gw[k], nw[k]), uu = unpack_u(uw[k], nw[k]);
               const float d0 = __uint_as_float(d[8 * j + 2 * k]);
               const float d1 = __uint_as_float(d[8 * j + 2 * k + 1]);
               float v0, s0, v1, s1;
@@ -515,7 +535,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
             }
             ptx::bulk_commit_group();
           }
-          if (kGradSlots == 1 && c + 1 < kGradChunks) load_inputs(c + 1);
         }
       } else if (w.part >= 0) {
         // fp32 partial sums, 32 columns at a time.

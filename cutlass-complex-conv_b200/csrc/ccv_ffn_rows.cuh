@@ -104,7 +104,7 @@ struct RowsParams {
   const uint16_t* x;       // [rows][k]: tokens (gate) or h (down)
   int64_t x_stride;
   const uint16_t *w0, *w1; // gate and up [out][k]; down [out][k] and null
-  uint16_t *out, *g, *u;   // h, g, u (g, u null without saving); y
+  uint16_t *out, *g, *u, *next;  // h and the planes of g and u (null without saving); y
   int64_t out_stride;
   int rows, k, outputs;
   int blocks_per_cta;      // gate: groups of 8 outputs per block
@@ -167,8 +167,10 @@ __global__ void __launch_bounds__(kRowsThreads)
         // Outputs past the last one have g = u = 0 and write the zero padding.
         reinterpret_cast<T*>(p.out)[at] = from_f32<T>(value * u);
         if (p.g != nullptr) {
-          reinterpret_cast<T*>(p.g)[at] = from_f32<T>(g);
-          reinterpret_cast<T*>(p.u)[at] = from_f32<T>(u);
+          const uint32_t gb = __float_as_uint(g), ub = __float_as_uint(u);
+          p.g[at] = static_cast<uint16_t>(gb >> 16);
+          p.u[at] = static_cast<uint16_t>(ub >> 16);
+          p.next[at] = static_cast<uint16_t>(next_bytes(gb, ub, gb, ub));
         }
       }
     }
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(kRowsThreads)
       if (m < p.rows) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int r = 0; r < size; ++r) {
-          const float4 q = ptx::ld_shared_cluster_v4(ptx::mapa_shared(ptx::smem_u32(sum + 4 * e), r));
+          const float4 q = ptx::ld_shared_cluster_v4_ordered(ptx::mapa_shared(ptx::smem_u32(sum + 4 * e), r));
           v.x += q.x;
           v.y += q.y;
           v.z += q.z;

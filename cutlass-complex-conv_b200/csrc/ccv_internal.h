@@ -211,7 +211,7 @@ struct FfnForward {
   int64_t x_stride;
   const void *w_gate, *w_up, *w_down;
   void* y;
-  void* saved;  // h, g, u planes for the backward pass, or null
+  void* saved;  // four planes for the backward pass (h; g and u to 24 bits), or null
   // Where a row length is a multiple of 8 elements its matrices are read by
   // TMA in place: bases 16-byte aligned, row strides multiples of 8.
 };

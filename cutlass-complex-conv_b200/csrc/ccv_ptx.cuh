@@ -445,6 +445,16 @@ __device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t addr) {
   return v;
 }
 
+// The same, kept in order with the barriers around it by the compiler too
+// (several may still be in flight).
+__device__ __forceinline__ float4 ld_shared_cluster_v4_ordered(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+
 // Cluster-wide barrier.  The non-.aligned forms count threads, so a warp
 // whose lanes arrive at different times (one lane ran a role loop alone) is
 // still waited for in full.

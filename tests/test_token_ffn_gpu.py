@@ -66,6 +66,34 @@ def test_larger(rows, features, hidden):
     _check(*_inputs(rows, features, hidden, seed=rows), "silu")
 
 
+@pytest.fixture
+def switches(monkeypatch):
+    """Sets the library's CCV_* switches for one test."""
+    from complex_conv2d import _C
+
+    def set_to(**kw):
+        for k, v in kw.items():
+            monkeypatch.setenv(k, str(v))
+        _C.reload_config()
+
+    yield set_to
+    monkeypatch.undo()
+    _C.reload_config()
+
+
+@pytest.mark.parametrize("env", [
+    dict(CCV_FFN_BN=128), dict(CCV_FFN_BN=256), dict(CCV_FFN_BN=256, CCV_FFN_SPLITS=3),
+    dict(CCV_FFN_BN=128, CCV_FFN_SPLITS=5), dict(CCV_FFN_SPLITS=1)],
+    ids=lambda e: "-".join(f"{k[8:]}{v}" for k, v in e.items()))
+@pytest.mark.parametrize("rows, features, hidden", [(33, 64, 136), (300, 200, 1000), (1000, 264, 600),
+                                                    (5000, 328, 1032), (257, 131, 77)])
+def test_every_kernel(rows, features, hidden, env, switches):
+    """Each tile width and the split of the last wave, on shapes they would
+    not all be chosen for."""
+    switches(**env)
+    _check(*_inputs(rows, features, hidden, seed=hidden), "gelu")
+
+
 def test_no_rows():
     x, wg, wu, wd, dy = _inputs(0, 64, 96)
     y, saved = cc.gated_feed_forward_with_saved(x, wg, wu, wd)
