@@ -269,10 +269,10 @@ struct Matrix {
   int64_t inner = 0, outer = 0, ld = 0;
 };
 
-template <typename T, int MODE, int BN, bool A_MN, bool B_MN>
+template <typename T, int MODE, int BN, bool A_MN, bool B_MN, int ACT>
 int launch_variant(const GemmParams& prm, cudaStream_t stream) {
   using C = ffn::Config<MODE, BN>;
-  auto kern = ffn::ffn_gemm_kernel<T, MODE, BN, A_MN, B_MN>;
+  auto kern = ffn::ffn_gemm_kernel<T, MODE, BN, A_MN, B_MN, ACT>;
   static std::once_flag once[64];
   static int max_clusters[64] = {};
   int dev = 0;
@@ -300,14 +300,24 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
                   "gated feed-forward product");
 }
 
-template <int MODE, bool A_MN, bool B_MN>
-int launch_product(const GemmParams& prm, int dtype, int bn, cudaStream_t stream) {
-  if (dtype == CCV_DTYPE_BF16) {
-    return bn == 256 ? launch_variant<__nv_bfloat16, MODE, 256, A_MN, B_MN>(prm, stream)
-                     : launch_variant<__nv_bfloat16, MODE, 128, A_MN, B_MN>(prm, stream);
+template <typename T, int MODE, bool A_MN, bool B_MN>
+int launch_typed(const GemmParams& prm, int bn, int act, cudaStream_t stream) {
+  constexpr int kSilu = CCV_ACTIVATION_SILU, kGelu = CCV_ACTIVATION_GELU;
+  if constexpr (MODE != ffn::PLAIN) {
+    if (act == kGelu) {
+      return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
+                       : launch_variant<T, MODE, 128, A_MN, B_MN, kGelu>(prm, stream);
+    }
   }
-  return bn == 256 ? launch_variant<__half, MODE, 256, A_MN, B_MN>(prm, stream)
-                   : launch_variant<__half, MODE, 128, A_MN, B_MN>(prm, stream);
+  return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kSilu>(prm, stream)
+                   : launch_variant<T, MODE, 128, A_MN, B_MN, kSilu>(prm, stream);
+}
+
+template <int MODE, bool A_MN, bool B_MN>
+int launch_product(const GemmParams& prm, int dtype, int bn, int act, cudaStream_t stream) {
+  return dtype == CCV_DTYPE_BF16
+             ? launch_typed<__nv_bfloat16, MODE, A_MN, B_MN>(prm, bn, act, stream)
+             : launch_typed<__half, MODE, A_MN, B_MN>(prm, bn, act, stream);
 }
 
 // One launch under construction.
@@ -316,18 +326,18 @@ struct Product {
   GemmParams prm = {};
   Plan plan;
   SplitSum sums = {};
-  int dtype;
+  int dtype, act;
   int64_t tiles = 0;
   int rc = CCV_OK;
 
-  Product(int dtype_, const Plan& plan_, int64_t k, int act) : plan(plan_), dtype(dtype_) {
+  Product(int dtype_, const Plan& plan_, int64_t k, int act_)
+      : plan(plan_), dtype(dtype_), act(act_) {
     prm.status = device_status_ptr();
     prm.problems = 1;
     prm.segments = 1;
     prm.ksteps = static_cast<int>(ceil_div(k, ffn::kStepK));
     prm.splits = plan.splits;
     prm.whole = static_cast<int>(plan.whole);
-    prm.act = act;
   }
   void operand_a(int i, const Matrix& x) {
     if (rc == CCV_OK) {
@@ -380,7 +390,7 @@ struct Product {
     const int64_t units = prm.whole + tail * plan.splits;
     if (units > 0x7fffffff) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
     prm.units = static_cast<int>(units);
-    const int launched_rc = launch_product<MODE, A_MN, B_MN>(prm, dtype, plan.bn, stream);
+    const int launched_rc = launch_product<MODE, A_MN, B_MN>(prm, dtype, plan.bn, act, stream);
     if (launched_rc != CCV_OK || tail == 0) return launched_rc;
     for (int i = 0; i < prm.problems; ++i) sums.tiles[i] = prm.tiles[i];
     sums.problems = prm.problems;

@@ -67,7 +67,6 @@ struct alignas(64) GemmParams {
   int whole, splits;
   int units;
   int save;     // GATE: store g and u too
-  int act;
 };
 
 template <int MODE, int BN>
@@ -149,8 +148,9 @@ __device__ __forceinline__ float rcp(float x) {
 // Stegun 7.1.26 (|error of erf| <= 1.5e-7), a polynomial times exp(-g^2/2),
 // the exponential its slope needs too.  Both errors, and the flush of values
 // below 2^-126 to zero, lie far below the 16-bit rounding of the result.
-__device__ __forceinline__ void activation(int act, float g, float& value, float& slope) {
-  if (act == CCV_ACTIVATION_SILU) {
+template <int ACT>
+__device__ __forceinline__ void activation(float g, float& value, float& slope) {
+  if constexpr (ACT == CCV_ACTIVATION_SILU) {
     const float s = rcp(1.f + ex2(g * -1.4426950408889634f));
     value = g * s;
     slope = fmaf(-value, s, value) + s;
@@ -244,7 +244,9 @@ __device__ __forceinline__ void publish() {
   __syncwarp();
 }
 
-template <typename T, int MODE, int BN, bool A_MN, bool B_MN>
+// ACT is a template parameter because a branch on it at each element kept the
+// compiler from interleaving elements: the gate epilogue took twice as long.
+template <typename T, int MODE, int BN, bool A_MN, bool B_MN, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MODE, BN>::kBlocksPerSm)
     ffn_gemm_kernel(const __grid_constant__ GemmParams p) {
   using C = Config<MODE, BN>;
@@ -479,8 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           };
           put([&](int k) {
             float v0, v1, slope;
-            activation(p.act, __uint_as_float(g[2 * k]), v0, slope);
-            activation(p.act, __uint_as_float(g[2 * k + 1]), v1, slope);
+            activation<ACT>(__uint_as_float(g[2 * k]), v0, slope);
+            activation<ACT>(__uint_as_float(g[2 * k + 1]), v1, slope);
             return pack2(v0 * __uint_as_float(v[2 * k]), v1 * __uint_as_float(v[2 * k + 1]), T());
           }, &p.out[0]);
           if (p.save) {
@@ -519,8 +521,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
               const float d0 = __uint_as_float(d[8 * j + 2 * k]);
               const float d1 = __uint_as_float(d[8 * j + 2 * k + 1]);
               float v0, s0, v1, s1;
-              activation(p.act, gg.x, v0, s0);
-              activation(p.act, gg.y, v1, s1);
+              activation<ACT>(gg.x, v0, s0);
+              activation<ACT>(gg.y, v1, s1);
               og[k] = pack2(d0 * uu.x * s0, d1 * uu.y * s1, T());
               ou[k] = pack2(d0 * v0, d1 * v1, T());
             }

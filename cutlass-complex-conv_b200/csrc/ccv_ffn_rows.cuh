@@ -162,7 +162,11 @@ __global__ void __launch_bounds__(kRowsThreads)
           u += part[w][f + 8][m];
         }
         float value, slope;
-        activation(p.act, g, value, slope);
+        if (p.act == CCV_ACTIVATION_SILU) {
+          activation<CCV_ACTIVATION_SILU>(g, value, slope);
+        } else {
+          activation<CCV_ACTIVATION_GELU>(g, value, slope);
+        }
         const int64_t at = m * p.out_stride + o0 + f;
         // Outputs past the last one have g = u = 0 and write the zero padding.
         reinterpret_cast<T*>(p.out)[at] = from_f32<T>(value * u);
