@@ -350,14 +350,18 @@ struct Product {
                      B_MN ? 64 : plan.bn / 2);
     }
   }
+  // Columns of an epilogue warp's stores.
+  int out_box() const {
+    return MODE == ffn::PLAIN || (MODE == ffn::GATE && plan.bn == 256) ? 64 : 32;
+  }
   void result(int i, void* base, int64_t m, int64_t n, int64_t ld) {
-    if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, MODE == ffn::PLAIN ? 64 : 32, 32);
+    if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, out_box(), 32);
     sums.out[i] = base;
     sums.ldo[i] = ld;
   }
-  // A plane of 16-bit words read or written 32 columns at a time.
+  // A plane of 16-bit words read or written beside the results.
   void plane(CUtensorMap* map, const void* base, int64_t m, int64_t n, int64_t ld) {
-    if (rc == CCV_OK) rc = encode_2d(map, dtype, base, n, m, ld, 32, 32);
+    if (rc == CCV_OK) rc = encode_2d(map, dtype, base, n, m, ld, out_box(), 32);
   }
   // Storage for the split tiles' parts (none without a split).
   void partials(void* base) {
@@ -378,6 +382,7 @@ struct Product {
     t.tiles_m = static_cast<int>(ceil_div(m, 256));
     t.tiles_n = static_cast<int>(ceil_div(n, MODE == ffn::GATE ? plan.bn / 2 : plan.bn));
     t.first = static_cast<int>(tiles);
+    t.band_inverse = static_cast<uint32_t>((1ULL << 32) / (ffn::kRasterRows * static_cast<uint64_t>(t.tiles_n)));
     tiles += static_cast<int64_t>(t.tiles_m) * t.tiles_n;
     prm.problems = i + 1;
   }

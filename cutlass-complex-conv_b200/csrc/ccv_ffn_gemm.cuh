@@ -48,6 +48,7 @@ struct Tiles {
   int m, n;              // extents of the result
   int tiles_m, tiles_n;
   int first;             // first tile
+  uint32_t band_inverse; // floor(2^32 / (kRasterRows * tiles_n))
 };
 
 struct alignas(64) GemmParams {
@@ -96,21 +97,31 @@ struct Unit {
 };
 
 // Problem, tile row and tile column of a tile.
-__host__ __device__ __forceinline__ void locate(const Tiles* tiles, int problems, int tile,
-                                                int& problem, int& tm, int& tn) {
+__device__ __forceinline__ void locate(const Tiles* tiles, int problems, int tile, int& problem,
+                                       int& tm, int& tn) {
   problem = 0;
   for (int i = 1; i < kMaxProblems; ++i) {
     if (i < problems && tile >= tiles[i].first) problem = i;
   }
   const Tiles& t = tiles[problem];
-  const int local = tile - t.first;
-  // Bands of kRasterRows tile rows, walked column by column.
-  const int band = local / (kRasterRows * t.tiles_n);
-  const int r = local - band * kRasterRows * t.tiles_n;
-  const int left = t.tiles_m - band * kRasterRows;
-  const int rows = left < kRasterRows ? left : kRasterRows;
-  tn = r / rows;
-  tm = band * kRasterRows + (r - tn * rows);
+  // Bands of kRasterRows tile rows, walked column by column.  The quotient by
+  // the inverse is exact or one too small.
+  const uint32_t local = static_cast<uint32_t>(tile - t.first);
+  const uint32_t size = static_cast<uint32_t>(kRasterRows * t.tiles_n);
+  uint32_t band = __umulhi(local, t.band_inverse);
+  uint32_t r = local - band * size;
+  if (r >= size) {
+    ++band;
+    r -= size;
+  }
+  const int left = t.tiles_m - static_cast<int>(band) * kRasterRows;
+  if (left >= kRasterRows) {
+    tn = static_cast<int>(r / kRasterRows);
+    tm = static_cast<int>(band * kRasterRows + r % kRasterRows);
+  } else {
+    tn = static_cast<int>(r) / left;
+    tm = static_cast<int>(band) * kRasterRows + static_cast<int>(r) - tn * left;
+  }
 }
 
 __device__ __forceinline__ Unit decode(const GemmParams& p, int u) {
@@ -310,51 +321,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0 && !skip) {
-      uint32_t g = 0;
+    // The whole warp walks the loop, so that addresses and coordinates stay
+    // in uniform registers, and one lane issues: with a loop of one lane alone
+    // a K step took 0.47 us to issue, more than its multiplication.
+    if (!skip) {
+      const bool issuer = ptx::elect_one() != 0;
+      const uint32_t lead_full = ptx::mapa_shared(full_bar(0), 0);
+      uint32_t stage = 0, parity = 1, issued = 0;
       bool abort = false;
       for (int u = cid; u < p.units && !abort; u += ncl) {
         const Unit w = decode(p, u);
         const int m0 = (2 * w.tm + static_cast<int>(rank)) * kRows;
         const int n0 = MODE == GATE ? w.tn * (BN / 2) : w.tn * BN + static_cast<int>(rank) * (BN / 2);
-        for (int ks = w.k0; ks < w.k1; ++ks, ++g) {
-          const int stage = static_cast<int>(g % C::kStages);
-          if (!ptx::mbar_wait_bounded(empty_bar(stage), ((g / C::kStages) & 1u) ^ 1u, p.status,
-                                      kTimeoutCode) ||
-              flags[1]) {
-            flags[1] = 1;
-            abort = true;
-            break;
-          }
-          if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * C::kStage);
-          const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0);
-          const int seg = ks >= p.ksteps ? 1 : 0;
-          const int k = (ks - seg * p.ksteps) * kStepK;
+        for (int seg = 0; seg < p.segments && !abort; ++seg) {
+          const int first = max(w.k0 - seg * p.ksteps, 0);
+          const int last = min(w.k1 - seg * p.ksteps, p.ksteps);
           const int map = p.problems > 1 ? w.problem : seg;
           const CUtensorMap* ma = &p.a[map];
           const CUtensorMap* mb = &p.b[MODE == GATE ? static_cast<int>(rank) : map];
-          const uint32_t sa = smem_base + stage * C::kStage;
-          const uint32_t sb = sa + kOperandA;
-          if constexpr (A_MN) {
-            ptx::tma_load_2d_pair(sa, ma, fb, m0, k);
-            ptx::tma_load_2d_pair(sa + 8192, ma, fb, m0 + 64, k);
-          } else {
-            ptx::tma_load_2d_pair(sa, ma, fb, k, m0);
-          }
-          if constexpr (B_MN) {
-#pragma unroll
-            for (int i = 0; i < BN / 128; ++i) {
-              ptx::tma_load_2d_pair(sb + 8192 * i, mb, fb, n0 + 64 * i, k);
+          for (int ks = first; ks < last; ++ks) {
+            if (!ptx::mbar_wait_bounded(empty_bar(stage), parity, p.status, kTimeoutCode)) {
+              flags[1] = 1;
+              abort = true;
+              break;
             }
-          } else {
-            ptx::tma_load_2d_pair(sb, mb, fb, k, n0);
+            const uint32_t fb = lead_full + 8u * stage;
+            const uint32_t sa = smem_base + stage * C::kStage;
+            const uint32_t sb = sa + kOperandA;
+            const int k = ks * kStepK;
+            if (issuer) {
+              if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * C::kStage);
+              if constexpr (A_MN) {
+                ptx::tma_load_2d_pair(sa, ma, fb, m0, k);
+                ptx::tma_load_2d_pair(sa + 8192, ma, fb, m0 + 64, k);
+              } else {
+                ptx::tma_load_2d_pair(sa, ma, fb, k, m0);
+              }
+              if constexpr (B_MN) {
+#pragma unroll
+                for (int i = 0; i < BN / 128; ++i) {
+                  ptx::tma_load_2d_pair(sb + 8192 * i, mb, fb, n0 + 64 * i, k);
+                }
+              } else {
+                ptx::tma_load_2d_pair(sb, mb, fb, k, n0);
+              }
+            }
+            ++issued;
+            if (++stage == C::kStages) {
+              stage = 0;
+              parity ^= 1u;
+            }
           }
         }
       }
       if (leader) {
         // Drain: every issued stage's bytes (both CTAs) have landed.
-        for (uint32_t j = 0; j < static_cast<uint32_t>(C::kStages) && j < g; ++j) {
-          const uint32_t gg = g - 1 - j;
+        for (uint32_t j = 0; j < static_cast<uint32_t>(C::kStages) && j < issued; ++j) {
+          const uint32_t gg = issued - 1 - j;
           ptx::mbar_wait_bounded(full_bar(static_cast<int>(gg % C::kStages)),
                                  (gg / C::kStages) & 1u, p.status, kTimeoutCode);
         }
@@ -362,47 +385,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader && lane == 0 && !skip) {
-      constexpr uint32_t idesc = ptx::idesc_f16(2 * kRows, BN, kIsBf16<T>, A_MN,
-                                                B_MN);
-      uint32_t g = 0;
+    if (leader && !skip) {
+      constexpr uint32_t idesc = ptx::idesc_f16(2 * kRows, BN, kIsBf16<T>, A_MN, B_MN);
+      const bool issuer = ptx::elect_one() != 0;
+      // Descriptors of stage 0; a stage or K step further is an addition to
+      // the address field (16-byte units).
+      const uint64_t da0 = A_MN ? ptx::desc_mnmajor_sw128(smem_base, 8192)
+                                : ptx::desc_kmajor_sw128(smem_base);
+      const uint64_t db0 = B_MN ? ptx::desc_mnmajor_sw128(smem_base + kOperandA, 8192)
+                                : ptx::desc_kmajor_sw128(smem_base + kOperandA);
+      constexpr uint32_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
+      uint32_t stage = 0, parity = 0;
       int i = 0;
       bool abort = false;
       for (int u = cid; u < p.units && !abort; u += ncl, ++i) {
         const Unit w = decode(p, u);
         const int buf = i & 1;
-        const uint32_t use = static_cast<uint32_t>(i >> 1);
-        if (!ptx::mbar_wait_bounded(tempty_bar(buf), (use & 1u) ^ 1u, p.status, kTimeoutCode)) {
+        if (!ptx::mbar_wait_bounded(tempty_bar(buf), ((i >> 1) & 1u) ^ 1u, p.status, kTimeoutCode)) {
           flags[1] = 1;
           break;
         }
         ptx::tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(buf * BN);
-        for (int ks = w.k0; ks < w.k1; ++ks, ++g) {
-          const int stage = static_cast<int>(g % C::kStages);
-          if (!ptx::mbar_wait_bounded(full_bar(stage), (g / C::kStages) & 1u, p.status,
-                                      kTimeoutCode)) {
+        for (int ks = w.k0; ks < w.k1; ++ks) {
+          if (!ptx::mbar_wait_bounded(full_bar(stage), parity, p.status, kTimeoutCode)) {
             flags[1] = 1;
             abort = true;
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t sa = smem_base + stage * C::kStage;
-          const uint32_t sb = sa + kOperandA;
+          const uint64_t da = da0 + stage * (C::kStage / 16);
+          const uint64_t db = db0 + stage * (C::kStage / 16);
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < kStepK / 16; ++kk) {
-            const uint64_t da = A_MN ? ptx::desc_mnmajor_sw128(sa + kk * 2048, 8192)
-                                     : ptx::desc_kmajor_sw128(sa + kk * 32);
-            const uint64_t db = B_MN ? ptx::desc_mnmajor_sw128(sb + kk * 2048, 8192)
-                                     : ptx::desc_kmajor_sw128(sb + kk * 32);
-            ptx::mma_f16_pair(d, da, db, idesc, (ks != w.k0 || kk != 0) ? 1u : 0u);
+            for (int kk = 0; kk < kStepK / 16; ++kk) {
+              ptx::mma_f16_pair(d, da + kk * kStepA, db + kk * kStepB, idesc,
+                                (ks != w.k0 || kk != 0) ? 1u : 0u);
+            }
+            ptx::mma_commit_pair(empty_bar(stage));
           }
-          ptx::mma_commit_pair(empty_bar(stage));
+          if (++stage == C::kStages) {
+            stage = 0;
+            parity ^= 1u;
+          }
         }
-        ptx::mma_commit_pair(tfull_bar(buf));
+        if (issuer) ptx::mma_commit_pair(tfull_bar(buf));
       }
       // All issued MMAs complete before teardown.
-      ptx::mma_commit_pair(done_bar);
+      if (issuer) ptx::mma_commit_pair(done_bar);
       ptx::mbar_wait_bounded(done_bar, 0, p.status, kTimeoutCode);
     }
     __syncwarp();
@@ -452,45 +482,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
       ptx::tc_fence_after();
       if (!ok) flags[1] = 1;
       const bool store = ok && !flags[1];
+      // This warp has read its part of the accumulator: the MMA issuer may
+      // overwrite it once every epilogue warp says so.
+      auto release = [&]() {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster_relaxed(buf == 0 ? tempty0 : tempty1);
+      };
       if constexpr (MODE == GATE) {
-        // BN / 4 outputs per warp, 32 at a time.
-#pragma unroll 1
-        for (int c = 0; c < BN / 4; c += 32) {
-          const int fc = half * (BN / 4) + c;
-          uint32_t g[32], v[32];
-          ptx::tmem_ld_32x32b_x32(acc + fc, g);
-          ptx::tmem_ld_32x32b_x32(acc + BN / 2 + fc, v);
-          ptx::tmem_wait_ld();
-          ptx::reg_fence(g);
-          ptx::reg_fence(v);
-          const int col = w.tn * (BN / 2) + fc;
-          const bool in = store && rows_in && col < t.n;
-          // word(k): elements 2 k and 2 k + 1.
-          auto put = [&](auto&& word, const CUtensorMap* map) {
-            const uint32_t slot = ring2.take(lane);
+        // BN / 4 outputs per warp (64 or 32), all at once: rows of 128 (64)
+        // bytes for the stores.
+        constexpr int kOut = BN / 4;
+        const int fc = half * kOut;
+        uint32_t g[kOut], v[kOut];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              st_shared_v4(slot64(slot, lane, j), word(4 * j), word(4 * j + 1), word(4 * j + 2),
-                           word(4 * j + 3));
-            }
-            publish();
-            if (lane == 0) {
-              if (in) ptx::tma_store_2d(map, slot, col, row0);
-              ptx::bulk_commit_group();
-            }
-          };
-          put([&](int k) {
-            float v0, v1, slope;
-            activation<ACT>(__uint_as_float(g[2 * k]), v0, slope);
-            activation<ACT>(__uint_as_float(g[2 * k + 1]), v1, slope);
-            return pack2(v0 * __uint_as_float(v[2 * k]), v1 * __uint_as_float(v[2 * k + 1]), T());
-          }, &p.out[0]);
-          if (p.save) {
-            put([&](int k) { return high_halves(g[2 * k], g[2 * k + 1]); }, &p.out[1]);
-            put([&](int k) { return high_halves(v[2 * k], v[2 * k + 1]); }, &p.out[2]);
-            put([&](int k) { return next_bytes(g[2 * k], v[2 * k], g[2 * k + 1], v[2 * k + 1]); },
-                &p.out[3]);
+        for (int c = 0; c < kOut; c += 32) {
+          ptx::tmem_ld_32x32b_x32(acc + fc + c, *reinterpret_cast<uint32_t(*)[32]>(g + c));
+          ptx::tmem_ld_32x32b_x32(acc + BN / 2 + fc + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+        }
+        ptx::tmem_wait_ld();
+        ptx::reg_fence(g);
+        ptx::reg_fence(v);
+        release();
+        const int col = w.tn * (BN / 2) + fc;
+        const bool in = store && rows_in && col < t.n;
+        // word(k): elements 2 k and 2 k + 1.
+        auto put = [&](auto&& word, const CUtensorMap* map) {
+          const uint32_t slot = kOut == 64 ? ring4.take(lane) : ring2.take(lane);
+#pragma unroll
+          for (int j = 0; j < kOut / 8; ++j) {
+            st_shared_v4(kOut == 64 ? slot128(slot, lane, j) : slot64(slot, lane, j), word(4 * j),
+                         word(4 * j + 1), word(4 * j + 2), word(4 * j + 3));
           }
+          publish();
+          if (lane == 0) {
+            if (in) ptx::tma_store_2d(map, slot, col, row0);
+            ptx::bulk_commit_group();
+          }
+        };
+        put([&](int k) {
+          float v0, v1, slope;
+          activation<ACT>(__uint_as_float(g[2 * k]), v0, slope);
+          activation<ACT>(__uint_as_float(g[2 * k + 1]), v1, slope);
+          return pack2(v0 * __uint_as_float(v[2 * k]), v1 * __uint_as_float(v[2 * k + 1]), T());
+        }, &p.out[0]);
+        if (p.save) {
+          put([&](int k) { return high_halves(g[2 * k], g[2 * k + 1]); }, &p.out[1]);
+          put([&](int k) { return high_halves(v[2 * k], v[2 * k + 1]); }, &p.out[2]);
+          put([&](int k) { return next_bytes(g[2 * k], v[2 * k], g[2 * k + 1], v[2 * k + 1]); },
+              &p.out[3]);
         }
       } else if constexpr (MODE == GRAD) {
 #pragma unroll 1
@@ -500,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           const uint32_t slot = staging + (loads % kGradSlots) * kGradBytes;
           uint32_t d[32];
           ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 32, d);
-          ok = ptx::mbar_wait_bounded_backoff(loaded + 8u * (loads % kGradSlots), (loads / kGradSlots) & 1u,
+          ok = ptx::mbar_wait_bounded(loaded + 8u * (loads % kGradSlots), (loads / kGradSlots) & 1u,
                                               p.status, kTimeoutCode) && ok;
           ++loads;
           if (!ok) flags[1] = 1;
@@ -589,10 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           }
         }
       }
-      // This warp is done with the accumulator: release it to the MMA issuer.
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster_relaxed(buf == 0 ? tempty0 : tempty1);
+      if constexpr (MODE != GATE) release();
       if (!ok) break;
     }
     // Output stores still in flight complete before the CTA exits.
