@@ -283,7 +283,7 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
     if (err != cudaSuccess) return;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(4 * 148, 1, 1);
-    cfg.blockDim = dim3(ffn::kThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) {
@@ -295,7 +295,7 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
   });
   if (err != cudaSuccess) return cuda_error(err, "cudaFuncSetAttribute(ffn)");
   const int clusters = std::min(prm.units, std::max(1, max_clusters[dev & 63]));
-  return launched(launch_kernel(kern, dim3(2 * clusters), dim3(ffn::kThreads), C::kSmem, stream, 0,
+  return launched(launch_kernel(kern, dim3(2 * clusters), dim3(C::kThreads), C::kSmem, stream, 0,
                                 prm),
                   "gated feed-forward product");
 }
@@ -352,7 +352,7 @@ struct Product {
   }
   // Columns of an epilogue warp's stores.
   int out_box() const {
-    return MODE == ffn::PLAIN || (MODE == ffn::GATE && plan.bn == 256) ? 64 : 32;
+    return MODE == ffn::PLAIN ? 64 : 32;
   }
   void result(int i, void* base, int64_t m, int64_t n, int64_t ld) {
     if (rc == CCV_OK) rc = encode_2d(&prm.out[i], dtype, base, n, m, ld, out_box(), 32);

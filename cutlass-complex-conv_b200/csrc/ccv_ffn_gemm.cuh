@@ -16,12 +16,12 @@
 // they lie and multiplied through the M/N-innermost descriptor form: nothing
 // is transposed.
 //
-// Two accumulators in TMEM let eight epilogue warps work on one tile while
+// Two accumulators in TMEM let the epilogue warps work on one tile while
 // the next is multiplied; they pass their results through swizzled
 // shared-memory slots to TMA stores, which clip the ragged edges.
 //
-// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue (even CTA), 2-9
-// epilogue (quarter of the rows = warp % 4, half of the columns).
+// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue (even CTA), then the
+// epilogue (quarter of the rows = warp % 4, a group of the columns).
 #pragma once
 
 #include <cuda.h>
@@ -38,8 +38,6 @@ enum Mode { GATE, PLAIN, GRAD };
 constexpr int kRows = 128;        // rows of one CTA's tile
 constexpr int kStepK = 64;        // reduction elements per pipeline stage: 128-byte rows
 constexpr int kOperandA = kRows * kStepK * 2;
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kMaxProblems = 3;
 constexpr int kRasterRows = 8;    // tile rows walked together (operand reuse in L2)
 constexpr int kTimeoutCode = CCV_ERR_DEVICE_TIMEOUT;
@@ -74,13 +72,18 @@ template <int MODE, int BN>
 struct Config {
   static constexpr int kOperandB = BN / 2 * kStepK * 2;
   static constexpr int kStage = kOperandA + kOperandB;
+  // The gate epilogue is bound by issue slots and latency: sixteen warps work
+  // on a 256-wide tile (39 -> 35 us at 25088 x 256 -> 2 x 1024 GELU).
+  static constexpr int kEpiWarps = MODE == GATE && BN == 256 ? 16 : 8;
+  static constexpr int kThreads = 64 + 32 * kEpiWarps;
+  static constexpr int kGroups = kEpiWarps / 4;  // warps that share a row quarter's columns
   // BN = 256: one block per SM.  BN = 128, for problems of few tiles: few
   // stages and little staging, so that two blocks share an SM and the next
   // launch's blocks start up beside this one's.  GRAD trades a stage for room
   // to load its inputs a chunk ahead.
   static constexpr int kBlocksPerSm = BN == 256 || MODE == GRAD ? 1 : 2;
-  static constexpr int kWarpStaging = MODE == GRAD ? 12288 : (BN == 256 ? 8192 : 4096);
-  static constexpr int kStaging = kEpiWarps * kWarpStaging;
+  static constexpr int kStaging = MODE == GRAD ? 98304 : (BN == 256 ? 65536 : 32768);
+  static constexpr int kWarpStaging = kStaging / kEpiWarps;
   static constexpr int kStages = MODE == GRAD ? (BN == 256 ? 4 : 5) : (BN == 256 ? 5 : 3);
   static constexpr int kStagingOffset = kStages * kStage;
   static constexpr int kBarOffset = kStagingOffset + kStaging;
@@ -258,7 +261,7 @@ __device__ __forceinline__ void publish() {
 // ACT is a template parameter because a branch on it at each element kept the
 // compiler from interleaving elements: the gate epilogue took twice as long.
 template <typename T, int MODE, int BN, bool A_MN, bool B_MN, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MODE, BN>::kBlocksPerSm)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kThreads, Config<MODE, BN>::kBlocksPerSm)
     ffn_gemm_kernel(const __grid_constant__ GemmParams p) {
   using C = Config<MODE, BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -267,7 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
   // full[S] (even CTA), empty[S], tfull[2], tempty[2] (even CTA), done,
   // loaded[2][8] (GRAD: an epilogue warp's g and u), the TMEM address, flags.
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 5 + 2 * kEpiWarps);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * C::kStages + 5 + 2 * C::kEpiWarps);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_holder + 1);  // [0] skip, [1] abort
 
   const int warp = threadIdx.x >> 5;
@@ -293,10 +296,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
     }
     for (int b = 0; b < 2; ++b) {
       ptx::mbar_init(tfull_bar(b), 1);
-      ptx::mbar_init(tempty_bar(b), 2 * kEpiWarps);  // both CTAs' epilogue warps
+      ptx::mbar_init(tempty_bar(b), 2 * C::kEpiWarps);  // both CTAs' epilogue warps
     }
     ptx::mbar_init(done_bar, 1);
-    for (int i = 0; i < 2 * kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
+    for (int i = 0; i < 2 * C::kEpiWarps; ++i) ptx::mbar_init(loaded_bar0 + 8u * i, 1);
     ptx::fence_mbar_init();
   }
   // A timeout reported by an earlier kernel: this one exits without work.
@@ -440,7 +443,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
     // ------------------------------------------------------------ epilogue
     const int e = warp - 2;
     const int quarter = warp & 3;
-    const int half = e >> 2;
+    const int group = e >> 2;  // of the columns
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t staging = smem_base + C::kStagingOffset + e * C::kWarpStaging;
     const uint32_t loaded = loaded_bar0 + 16u * e;
@@ -463,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
       // replace the high halves there and are stored from there.
       constexpr int kGradChunks = BN / 2 / 32;
       constexpr uint32_t kGradBytes = 3 * 2048, kGradSlots = 2;
-      const int grad_col = w.tn * BN + half * (BN / 2);
+      const int grad_col = w.tn * BN + group * (BN / 2);
       auto load_inputs = [&](int c) {
         if (lane == 0) {
           ptx::bulk_wait_read_all();  // the slot's last results have been read
@@ -490,16 +493,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
         if (lane == 0) ptx::mbar_arrive_cluster_relaxed(buf == 0 ? tempty0 : tempty1);
       };
       if constexpr (MODE == GATE) {
-        // BN / 4 outputs per warp (64 or 32), all at once: rows of 128 (64)
-        // bytes for the stores.
-        constexpr int kOut = BN / 4;
-        const int fc = half * kOut;
-        uint32_t g[kOut], v[kOut];
-#pragma unroll
-        for (int c = 0; c < kOut; c += 32) {
-          ptx::tmem_ld_32x32b_x32(acc + fc + c, *reinterpret_cast<uint32_t(*)[32]>(g + c));
-          ptx::tmem_ld_32x32b_x32(acc + BN / 2 + fc + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
-        }
+        static_assert(BN / 2 / C::kGroups == 32, "32 outputs per warp");
+        const int fc = group * 32;
+        uint32_t g[32], v[32];
+        ptx::tmem_ld_32x32b_x32(acc + fc, g);
+        ptx::tmem_ld_32x32b_x32(acc + BN / 2 + fc, v);
         ptx::tmem_wait_ld();
         ptx::reg_fence(g);
         ptx::reg_fence(v);
@@ -508,11 +506,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
         const bool in = store && rows_in && col < t.n;
         // word(k): elements 2 k and 2 k + 1.
         auto put = [&](auto&& word, const CUtensorMap* map) {
-          const uint32_t slot = kOut == 64 ? ring4.take(lane) : ring2.take(lane);
+          const uint32_t slot = ring2.take(lane);
 #pragma unroll
-          for (int j = 0; j < kOut / 8; ++j) {
-            st_shared_v4(kOut == 64 ? slot128(slot, lane, j) : slot64(slot, lane, j), word(4 * j),
-                         word(4 * j + 1), word(4 * j + 2), word(4 * j + 3));
+          for (int j = 0; j < 4; ++j) {
+            st_shared_v4(slot64(slot, lane, j), word(4 * j), word(4 * j + 1), word(4 * j + 2),
+                         word(4 * j + 3));
           }
           publish();
           if (lane == 0) {
@@ -539,7 +537,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           const int col = grad_col + c * 32;
           const uint32_t slot = staging + (loads % kGradSlots) * kGradBytes;
           uint32_t d[32];
-          ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c * 32, d);
+          ptx::tmem_ld_32x32b_x32(acc + group * (BN / 2) + c * 32, d);
           ok = ptx::mbar_wait_bounded(loaded + 8u * (loads % kGradSlots), (loads / kGradSlots) & 1u,
                                               p.status, kTimeoutCode) && ok;
           ++loads;
@@ -583,7 +581,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
 #pragma unroll 1
         for (int c = 0; c < BN / 2; c += 32) {
           uint32_t d[32];
-          ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c, d);
+          ptx::tmem_ld_32x32b_x32(acc + group * (BN / 2) + c, d);
           ptx::tmem_wait_ld();
           ptx::reg_fence(d);
           const uint32_t slot = ring4.take(lane);
@@ -594,7 +592,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
           publish();
           if (lane == 0) {
             if (store && rows_in) {
-              ptx::tma_store_3d(&p.partial, slot, half * (BN / 2) + c,
+              ptx::tma_store_3d(&p.partial, slot, group * (BN / 2) + c,
                                 static_cast<int>(rank) * kRows + quarter * 32, w.part);
             }
             ptx::bulk_commit_group();
@@ -603,12 +601,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Config<MOD
       } else {
 #pragma unroll 1
         for (int c = 0; c < BN / 2; c += 64) {
-          const int col = w.tn * BN + half * (BN / 2) + c;
+          const int col = w.tn * BN + group * (BN / 2) + c;
           const uint32_t slot = ring4.take(lane);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t d[32];
-            ptx::tmem_ld_32x32b_x32(acc + half * (BN / 2) + c + h * 32, d);
+            ptx::tmem_ld_32x32b_x32(acc + group * (BN / 2) + c + h * 32, d);
             ptx::tmem_wait_ld();
             ptx::reg_fence(d);
 #pragma unroll
