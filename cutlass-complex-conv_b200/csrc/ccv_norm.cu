@@ -18,12 +18,13 @@
 // rows there, reading nothing twice; blocks leave fp32 partial sums that a
 // second launch adds in block order (deterministic).
 //
-// Dense rows whose width no vector divides start at any element of a vector.
-// A group's rows are then a multiple of V rows apart, so they all start at
-// the same one, and the group's vectors are shifted by it: loads stay whole
-// aligned vectors, whose first and last elements may belong to the row's
-// neighbours and are ignored (SHIFT).  Other layouts take single elements,
-// and rows wider than 8192 the kernels further down.
+// Rows that 16-byte vectors do not divide go in pairs of elements where those
+// divide them.  Dense rows of odd width start at any element of a vector: a
+// group's rows are then a multiple of V rows apart, so they all start at the
+// same one, and the group's vectors are shifted by it; the first and the last
+// may hold elements of the row's neighbours, which a bit mask excludes
+// (SHIFT).  Other layouts take single elements, and rows wider than 8192 the
+// kernels further down.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -110,6 +111,8 @@ struct Held {
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
       } else if constexpr (kPiece == 8) {
         asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at), "r"(0) : "memory");
+      } else if constexpr (kPiece == 4) {
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(0) : "memory");
       }
     }
   }
@@ -162,6 +165,26 @@ __device__ __forceinline__ void clip(Vec<T, V>& v, int c, int features) {
   }
 }
 
+// Bits of the elements of a thread's vectors that lie in the row (shifted
+// vectors: the first may begin in the row before, the last end in the next).
+template <int V>
+struct Inside {
+  uint32_t bits = 0;
+  __device__ __forceinline__ void add(int i, int c, int features) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (c + j >= 0 && c + j < features) bits |= 1u << (i * V + j);
+    }
+  }
+  __device__ __forceinline__ bool element(int i, int j) const {
+    return (bits >> (i * V + j) & 1u) != 0;
+  }
+  __device__ __forceinline__ bool whole(int i) const {
+    constexpr uint32_t all = (1u << V) - 1u;
+    return (bits >> (i * V) & all) == all;
+  }
+};
+
 // Ring stages for `bytes` per thread and row.
 template <int BYTES>
 constexpr int kRingStages =
@@ -178,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int VPT = Hx::kVpt;
   constexpr int S = kRingStages<Hx::kBytes>;
   extern __shared__ __align__(16) uint8_t ring[];
-  __shared__ float red[2 * (kThreads / 32)];
+  __shared__ float red[2 * (kThreads / 32) * 2];
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
   const int group = threadIdx.x / g;
@@ -188,6 +211,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
   const int shift = SHIFT ? static_cast<int>((first + group) * features % V) : 0;
   auto column = [&](int i) { return (i * g + lane) * V - shift; };
+  Inside<V> inside;
+  if (SHIFT) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) inside.add(i, column(i), features);
+  }
   const uint32_t ring_base = ptx::smem_u32(ring);
   const uint32_t stage_bytes = blockDim.x * Hx::kBytes;
   auto fetch = [&](int stage, int64_t r) {
@@ -225,69 +253,76 @@ __global__ void __launch_bounds__(kThreads, 1)
       bs[i][j] = in && b != nullptr ? to_f32(b[c + j]) : 0.f;
     }
   }
-  GroupSum<1> total{g, group, red};
+  GroupSum<2> total{g, group, red};
   const float n = static_cast<float>(features), inv = 1.f / n;
   int stage = 0;
-  // The block's groups walk together: every thread takes part in each sum.
-  for (int64_t r0 = first; r0 < rows; r0 += step) {
-    const int64_t r = r0 + group;
-    const bool live = r < rows;
-    copy_wait<S - 1>();
-    float v[VPT][V];
-    float sum[1] = {0.f};
+  // Two rows at a time: one exchange serves both sums, and the rows' chains of
+  // dependent operations overlap.  The block's groups walk together: every
+  // thread takes part in each sum.
+  for (int64_t r0 = first; r0 < rows; r0 += 2 * step) {
+    copy_wait<S - 2>();
+    float v[2][VPT][V];
+    float sum[2] = {0.f, 0.f}, mean[2], sq[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      Vec<Tx, V> q = Hx::read(ring + stage * stage_bytes, i);
-      const int c = column(i);
-      if (SHIFT && (c < 0 || c + V > features)) clip(q, c, features);
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[i][j] = to_f32(q.e[j]);
-        sum[0] += v[i][j];
-      }
-    }
-    fetch(stage, r + S * step);
-    stage = stage + 1 == S ? 0 : stage + 1;
-    total(sum);
-    const float mean = sum[0] / n;
-    float sq[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = column(i);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] -= mean;
-      if (SHIFT && (c < 0 || c + V > features)) {
+      for (int i = 0; i < VPT; ++i) {
+        const Vec<Tx, V> q = Hx::read(ring + stage * stage_bytes, i);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (c + j >= 0 && c + j < features) sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+          v[h][i][j] = !SHIFT || inside.element(i, j) ? to_f32(q.e[j]) : 0.f;
+          sum[h] += v[h][i][j];
         }
-      } else if (c < features) {
+      }
+      fetch(stage, r0 + group + (S + h) * step);
+      stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    total(sum);
 #pragma unroll
-        for (int j = 0; j < V; ++j) sq[0] = fmaf(v[i][j], v[i][j], sq[0]);
+    for (int h = 0; h < 2; ++h) {
+      mean[h] = sum[h] / n;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int c = column(i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[h][i][j] -= mean[h];
+        if (SHIFT) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (inside.element(i, j)) sq[h] = fmaf(v[h][i][j], v[h][i][j], sq[h]);
+          }
+        } else if (c < features) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) sq[h] = fmaf(v[h][i][j], v[h][i][j], sq[h]);
+        }
       }
     }
     total(sq);
-    const float rstd = rsqrtf(sq[0] * inv + eps);
-    if (!live) continue;
-    Ty* yr = y + r * features;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int c = column(i);
-      float o[V];
+    for (int h = 0; h < 2; ++h) {
+      const int64_t r = r0 + group + h * step;
+      if (r >= rows) break;
+      const float rstd = rsqrtf(sq[h] * inv + eps);
+      Ty* yr = y + r * features;
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = fmaf(v[i][j] * rstd, wt[i][j], bs[i][j]);
-      if (!SHIFT || (c >= 0 && c + V <= features)) {
-        if (c < features) store_vec<Ty, V>(yr + c, o);
-      } else {
+      for (int i = 0; i < VPT; ++i) {
+        const int c = column(i);
+        float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (c + j >= 0 && c + j < features) yr[c + j] = from_f32<Ty>(o[j]);
+        for (int j = 0; j < V; ++j) o[j] = fmaf(v[h][i][j] * rstd, wt[i][j], bs[i][j]);
+        if (SHIFT ? inside.whole(i) : c < features) {
+          store_vec<Ty, V>(yr + c, o);
+        } else if (SHIFT) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (inside.element(i, j)) yr[c + j] = from_f32<Ty>(o[j]);
+          }
         }
       }
-    }
-    if (lane == 0) {
-      if (mean_out != nullptr) mean_out[r] = mean;
-      if (rstd_out != nullptr) rstd_out[r] = rstd;
+      if (lane == 0) {
+        if (mean_out != nullptr) mean_out[r] = mean[h];
+        if (rstd_out != nullptr) rstd_out[r] = rstd;
+      }
     }
   }
 }
@@ -390,6 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (V > 1) {
         qx = Hx::read(ring + stage * stage_bytes, i);
         qg = Hy::read(ring + stage * stage_bytes + x_bytes, i);
+        // (A bit mask as in the forward kernel does not fit in the registers:
+        // 12545 x 1001 fp32 43 us against 36.)
         if (SHIFT && (c < 0 || c + V > features)) {
           clip(qx, c, features);
           clip(qg, c, features);
@@ -797,13 +834,13 @@ int launch_ring(const Rings& p, size_t smem, cudaStream_t stream, const char* wh
 template <typename Tx, typename Tw, typename Ty>
 struct RunForward {
   static constexpr int V = kWide<Tx>;
-  template <bool SHIFT>
+  template <int W, bool SHIFT>
   static int ring(const NormForward& a, cudaStream_t stream) {
-    const int g = group_size(a.features + (SHIFT ? V - 1 : 0), kHeld, kThreads);
-    const Rings p = plan_rings(a.rows, g, SHIFT ? V : 1);
-    const size_t smem =
-        static_cast<size_t>(p.per_block) * g * Held<Tx, V>::kBytes * kRingStages<Held<Tx, V>::kBytes>;
-    return launch_ring<norm_forward_ring<Tx, Tw, Ty, V, SHIFT>>(
+    constexpr int bytes = Held<Tx, W>::kBytes;
+    const int g = group_size(a.features + (SHIFT ? W - 1 : 0), kHeld, kThreads);
+    const Rings p = plan_rings(a.rows, g, SHIFT ? W : 1);
+    const size_t smem = static_cast<size_t>(p.per_block) * g * bytes * kRingStages<bytes>;
+    return launch_ring<norm_forward_ring<Tx, Tw, Ty, W, SHIFT>>(
         p, smem, stream, "layer norm forward", static_cast<const Tx*>(a.x), a.x_stride,
         static_cast<const Tw*>(a.weight), static_cast<const Tw*>(a.bias), a.eps,
         static_cast<Ty*>(a.y), a.mean, a.rstd, a.rows, static_cast<int>(a.features), g);
@@ -821,11 +858,16 @@ struct RunForward {
   static int run(const NormForward& a, cudaStream_t stream) {
     const bool wide = vec_rows<Tx, V>(a.x, a.x_stride, a.features) &&
                       vec_rows<Ty, V>(a.y, a.features, a.features);
-    if (a.features <= kThreads * kHeld - V + 1) {
-      if (wide) return ring<false>(a, stream);
-      if (shifted_rows<Tx, V>(a.x, a.x_stride, a.features) &&
+    if (a.features <= kThreads * kHeld) {
+      if (wide) return ring<V, false>(a, stream);
+      if (vec_rows<Tx, 2>(a.x, a.x_stride, a.features) &&
+          vec_rows<Ty, 2>(a.y, a.features, a.features)) {
+        return ring<2, false>(a, stream);
+      }
+      if (a.features + V - 1 <= kThreads * kHeld &&
+          shifted_rows<Tx, V>(a.x, a.x_stride, a.features) &&
           shifted_rows<Ty, V>(a.y, a.features, a.features)) {
-        return ring<true>(a, stream);
+        return ring<V, true>(a, stream);
       }
     }
     if (a.features <= 32768) {
@@ -867,12 +909,15 @@ struct RunBackward {
     const int64_t d = a.features;
     int slices = 0;
     int rc = CCV_OK;
-    if (d <= kThreads * kHeld - V + 1) {
+    if (d <= kThreads * kHeld) {
       if (vec_rows<Tx, V>(x, a.x_stride, d) && vec_rows<Ty, V>(dy, a.dy_stride, d) &&
           vec_rows<Tx, V>(a.dx, d, d)) {
         rc = ring<V, false>(a, partial, &slices, stream);
-      } else if (shifted_rows<Tx, V>(x, a.x_stride, d) && shifted_rows<Ty, V>(dy, a.dy_stride, d) &&
-                 shifted_rows<Tx, V>(a.dx, d, d)) {
+      } else if (vec_rows<Tx, 2>(x, a.x_stride, d) && vec_rows<Ty, 2>(dy, a.dy_stride, d) &&
+                 vec_rows<Tx, 2>(a.dx, d, d)) {
+        rc = ring<2, false>(a, partial, &slices, stream);
+      } else if (d + V - 1 <= kThreads * kHeld && shifted_rows<Tx, V>(x, a.x_stride, d) &&
+                 shifted_rows<Ty, V>(dy, a.dy_stride, d) && shifted_rows<Tx, V>(a.dx, d, d)) {
         rc = ring<V, true>(a, partial, &slices, stream);
       } else {
         rc = ring<1, false>(a, partial, &slices, stream);
