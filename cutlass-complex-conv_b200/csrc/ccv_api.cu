@@ -319,7 +319,13 @@ int device_sm_count() {
   int dev = 0;
   if (current_device(&dev) != CCV_OK) return 148;
   std::lock_guard<std::mutex> lk(g_dev_mutex);
-  return g_sm_count[dev] > 0 ? g_sm_count[dev] : 148;
+  if (g_sm_count[dev] == 0) {
+    // A size query before the first launch: the plans of both must agree.
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    g_sm_count[dev] = sms;
+  }
+  return g_sm_count[dev];
 }
 
 int encode_tiled(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,

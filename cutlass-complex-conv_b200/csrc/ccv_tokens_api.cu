@@ -21,6 +21,16 @@ int guarded(Fn&& body) noexcept {
   }
 }
 
+// The same for a size query: 0 when it cannot be answered.
+template <typename Fn>
+size_t guarded_size(Fn&& body) noexcept {
+  try {
+    return body();
+  } catch (...) {
+    return 0;
+  }
+}
+
 int invalid(const char* msg) { return set_error(CCV_ERR_INVALID_ARGUMENT, msg); }
 
 bool aligned_to(const void* p, size_t bytes) {
@@ -123,8 +133,9 @@ int ccv_layer_norm_forward(const void* x, int x_dtype, int64_t x_row_stride, con
 }
 
 size_t ccv_layer_norm_backward_workspace_bytes(int64_t rows, int64_t features) {
-  if (rows < 0 || features <= 0 || rows > kMaxExtent || features > kMaxExtent) return 0;
-  return norm_backward_workspace_bytes(rows, features);
+  return guarded_size([&]() -> size_t {
+    return check_rows(rows, features) == CCV_OK ? norm_backward_workspace_bytes(rows, features) : 0;
+  });
 }
 
 int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, const void* x,
@@ -162,18 +173,23 @@ int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, 
 
 size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden) {
   const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
-  return check_ffn(s) == CCV_OK ? 4 * ffn_plane_bytes(s) : 0;
+  return guarded_size(
+      [&]() -> size_t { return check_ffn(s) == CCV_OK ? 4 * ffn_plane_bytes(s) : 0; });
 }
 
 size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden,
                                              int save) {
   const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
-  return check_ffn(s) == CCV_OK ? ffn_forward_workspace_bytes(s, save != 0) : 0;
+  return guarded_size([&]() -> size_t {
+    return check_ffn(s) == CCV_OK ? ffn_forward_workspace_bytes(s, save != 0) : 0;
+  });
 }
 
 size_t ccv_gated_ffn_backward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden) {
   const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
-  return check_ffn(s) == CCV_OK ? ffn_backward_workspace_bytes(s) : 0;
+  return guarded_size([&]() -> size_t {
+    return check_ffn(s) == CCV_OK ? ffn_backward_workspace_bytes(s) : 0;
+  });
 }
 
 int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gate,
