@@ -61,7 +61,8 @@ def test_widths_that_no_vector_divides(rows, features, hidden):
 
 
 @pytest.mark.parametrize("rows, features, hidden", [(6000, 256, 512), (1, 1024, 4096),
-                                                    (4, 2048, 5504), (2100, 512, 2048)])
+                                                    (4, 2048, 5504), (2100, 512, 2048),
+                                                    (25000, 128, 1000)])
 def test_larger(rows, features, hidden):
     _check(*_inputs(rows, features, hidden, seed=rows), "silu")
 
