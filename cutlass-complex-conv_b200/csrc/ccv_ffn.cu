@@ -46,28 +46,55 @@ struct Carver {
 };
 
 // ------------------------------------------------------------ small kernels
-// Rows of 16-bit elements from one pitch to another.
-__global__ void ffn_copy_rows(const uint16_t* __restrict__ src, int64_t src_pitch,
-                              uint16_t* __restrict__ dst, int64_t dst_pitch, int64_t rows,
-                              int cols) {
+// Matrices of 16-bit elements from one row pitch to another, all in one
+// launch (blockIdx.y is the matrix): a call with odd sizes copies up to five.
+struct RowCopy {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t src_pitch, dst_pitch, rows;
+  int cols;
+};
+struct RowCopies {
+  RowCopy m[5];
+  int count = 0;
+  void add(const void* src, int64_t src_pitch, void* dst, int64_t dst_pitch, int64_t rows,
+           int64_t cols) {
+    m[count++] = {static_cast<const uint16_t*>(src), static_cast<uint16_t*>(dst), src_pitch,
+                  dst_pitch, rows, static_cast<int>(cols)};
+  }
+};
+
+constexpr int kCopyAhead = 16;  // loads in flight per lane
+
+__global__ void __launch_bounds__(256) ffn_copy_rows(const RowCopies c) {
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-      dst[r * dst_pitch + c] = src[r * src_pitch + c];
+  const RowCopy& m = c.m[blockIdx.y];
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x * 8 + (threadIdx.x >> 5); r < m.rows; r += gridDim.x * 8) {
+    const uint16_t* src = m.src + r * m.src_pitch;
+    uint16_t* dst = m.dst + r * m.dst_pitch;
+    for (int k0 = lane; k0 < m.cols; k0 += 32 * kCopyAhead) {
+      uint16_t v[kCopyAhead];
+#pragma unroll
+      for (int i = 0; i < kCopyAhead; ++i) {
+        if (k0 + 32 * i < m.cols) v[i] = src[k0 + 32 * i];
+      }
+#pragma unroll
+      for (int i = 0; i < kCopyAhead; ++i) {
+        if (k0 + 32 * i < m.cols) dst[k0 + 32 * i] = v[i];
+      }
     }
   }
 }
 
-int copy_rows(const void* src, int64_t src_pitch, void* dst, int64_t dst_pitch, int64_t rows,
-              int64_t cols, cudaStream_t stream) {
-  if (rows == 0) return CCV_OK;
-  return launched(launch_kernel(ffn_copy_rows,
-                                dim3(static_cast<unsigned>(std::min<int64_t>(rows, 148 * 16))),
-                                dim3(128), 0, stream, 1, static_cast<const uint16_t*>(src),
-                                src_pitch, static_cast<uint16_t*>(dst), dst_pitch, rows,
-                                static_cast<int>(cols)),
-                  "row copy");
+int copy_rows(const RowCopies& c, cudaStream_t stream) {
+  if (c.count == 0) return CCV_OK;
+  int64_t most = 1;
+  for (int i = 0; i < c.count; ++i) most = std::max(most, c.m[i].rows);
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((most + 7) / 8, 148 * 8));
+  return launched(
+      launch_kernel(ffn_copy_rows, dim3(blocks, c.count), dim3(256), 0, stream, 1, c), "row copy");
 }
 
 struct SplitSum {
@@ -419,8 +446,8 @@ struct Padded {
   Matrix matrix() const {
     return {copy != nullptr ? copy : src, cols, rows, copy != nullptr ? padded(cols) : src_ld};
   }
-  int fill(cudaStream_t stream) const {
-    return copy != nullptr ? copy_rows(src, src_ld, copy, padded(cols), rows, cols, stream) : CCV_OK;
+  void fill(RowCopies& c) const {
+    if (copy != nullptr) c.add(src, src_ld, copy, padded(cols), rows, cols);
   }
 };
 
@@ -527,10 +554,10 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   }
   const Padded x{f.x, f.x_stride, m, d, p.x}, wg{f.w_gate, d, hid, d, p.w_gate},
       wu{f.w_up, d, hid, d, p.w_up}, wd{f.w_down, hid, d, hid, p.w_down};
-  for (const Padded* q : {&x, &wg, &wu, &wd}) {
-    const int rc = q->fill(stream);
-    if (rc != CCV_OK) return rc;
-  }
+  RowCopies copies;
+  for (const Padded* q : {&x, &wg, &wu, &wd}) q->fill(copies);
+  int rc = copy_rows(copies, stream);
+  if (rc != CCV_OK) return rc;
   void* h = saved != nullptr ? saved : p.h;
   {
     Product<ffn::GATE, false, false> g(s.dtype, p.gate, d, s.activation);
@@ -543,8 +570,7 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
       g.prm.save = 1;
     }
     g.problem(0, m, hid);
-    const int rc = g.launch(stream);
-    if (rc != CCV_OK) return rc;
+    if ((rc = g.launch(stream)) != CCV_OK) return rc;
   }
   Product<ffn::PLAIN, false, false> y(s.dtype, p.down, hid, 0);
   y.operand_a(0, {h, hid, m, fp});
@@ -552,9 +578,10 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   y.problem(0, m, d);
   y.partials(p.partial);
   y.result(0, p.y != nullptr ? p.y : f.y, m, d, p.y != nullptr ? padded(d) : d);
-  const int rc = y.launch(stream);
-  if (rc != CCV_OK || p.y == nullptr) return rc;
-  return copy_rows(p.y, padded(d), f.y, d, m, d, stream);
+  if ((rc = y.launch(stream)) != CCV_OK || p.y == nullptr) return rc;
+  RowCopies out;
+  out.add(p.y, padded(d), f.y, d, m, d);
+  return copy_rows(out, stream);
 }
 
 int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
@@ -578,11 +605,15 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
   const Padded dy{b.dy, b.dy_stride, m, d, p.dy}, x{b.x, b.x_stride, m, d, p.x},
       wg{b.w_gate, d, hid, d, p.w_gate}, wu{b.w_up, d, hid, d, p.w_up},
       wd{b.w_down, hid, d, hid, p.w_down};
-  int rc = dy.fill(stream);
-  if (rc == CCV_OK && (dw[0] != nullptr || dw[1] != nullptr)) rc = x.fill(stream);
-  if (rc == CCV_OK && need_grad) rc = wd.fill(stream);
-  if (rc == CCV_OK && b.dx != nullptr) rc = wg.fill(stream);
-  if (rc == CCV_OK && b.dx != nullptr) rc = wu.fill(stream);
+  RowCopies copies, out_copies;
+  dy.fill(copies);
+  if (dw[0] != nullptr || dw[1] != nullptr) x.fill(copies);
+  if (need_grad) wd.fill(copies);
+  if (b.dx != nullptr) {
+    wg.fill(copies);
+    wu.fill(copies);
+  }
+  int rc = copy_rows(copies, stream);
   if (rc != CCV_OK) return rc;
   if (need_grad) {
     Product<ffn::GRAD, false, true> g(s.dtype, p.grad, d, s.activation);
@@ -606,9 +637,7 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
     g.result(0, out, m, d, p.out_dx != nullptr ? padded(d) : d);
     g.partials(p.partial);
     if ((rc = g.launch(stream)) != CCV_OK) return rc;
-    if (p.out_dx != nullptr && (rc = copy_rows(out, padded(d), b.dx, d, m, d, stream)) != CCV_OK) {
-      return rc;
-    }
+    if (p.out_dx != nullptr) out_copies.add(out, padded(d), b.dx, d, m, d);
   }
   const Matrix left[3] = {{p.dg, hid, m, fp}, {p.du, hid, m, fp}, dy.matrix()};
   const Matrix right[3] = {x.matrix(), x.matrix(), {saved, hid, m, fp}};
@@ -624,15 +653,16 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
     g.result(count, out, e.m, e.n, p.out_dw[i] != nullptr ? padded(e.n) : e.n);
     ++count;
   }
-  if (count == 0) return CCV_OK;
-  g.partials(p.partial);
-  if ((rc = g.launch(stream)) != CCV_OK) return rc;
+  if (count > 0) {
+    g.partials(p.partial);
+    if ((rc = g.launch(stream)) != CCV_OK) return rc;
+  }
   for (int i = 0; i < 3; ++i) {
     if (dw[i] == nullptr || p.out_dw[i] == nullptr) continue;
     const Extent& e = p.dw_extent[i];
-    if ((rc = copy_rows(p.out_dw[i], padded(e.n), dw[i], e.n, e.m, e.n, stream)) != CCV_OK) return rc;
+    out_copies.add(p.out_dw[i], padded(e.n), dw[i], e.n, e.m, e.n);
   }
-  return CCV_OK;
+  return copy_rows(out_copies, stream);
 }
 
 }  // namespace ccv
