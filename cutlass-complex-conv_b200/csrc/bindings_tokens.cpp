@@ -231,6 +231,12 @@ FfnWeights check_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
 // Columns of a plane of the saved buffer (rows of whole 16-byte units).
 int64_t saved_width(int64_t hidden) { return (hidden + 7) / 8 * 8; }
 
+// Its planes: what the library asks for one row.
+int64_t saved_planes(int64_t features, int64_t hidden) {
+  return static_cast<int64_t>(ccv_gated_ffn_saved_bytes(1, features, hidden)) /
+         (2 * saved_width(hidden));
+}
+
 int activation_code(const std::string& name) {
   if (name == "silu") return CCV_ACTIVATION_SILU;
   TORCH_CHECK_VALUE(name == "gelu", "activation must be 'silu' or 'gelu', got '", name, "'");
@@ -252,7 +258,8 @@ std::tuple<torch::Tensor, torch::Tensor> gated_ffn_forward(torch::Tensor x, torc
   size_t saved_bytes = 0;
   if (save) {
     saved_bytes = ccv_gated_ffn_saved_bytes(r.rows, r.features, w.hidden);
-    saved = fresh({4, r.rows, saved_width(w.hidden)}, x.scalar_type(), x);
+    saved = fresh({saved_planes(r.features, w.hidden), r.rows, saved_width(w.hidden)},
+                  x.scalar_type(), x);
   }
   const size_t bytes = ccv_gated_ffn_forward_workspace_bytes(r.rows, r.features, w.hidden, save);
   auto ws = scratch(bytes, x);
@@ -280,7 +287,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn
   check_like(saved, x, "saved");
   const Rows rx = as_tma_rows(x), rdy = as_tma_rows(dy);
   TORCH_CHECK_VALUE(saved.scalar_type() == x.scalar_type() && saved.is_contiguous() &&
-                        saved.dim() == 3 && saved.size(0) == 4 && saved.size(1) == rx.rows &&
+                        saved.dim() == 3 && saved.size(0) == saved_planes(rx.features, w.hidden) && saved.size(1) == rx.rows &&
                         saved.size(2) == saved_width(w.hidden),
                     "saved must be what the forward call returned for these shapes");
   torch::Tensor dx, dg, du, dd;

@@ -212,6 +212,12 @@ int run_rows(const FfnForward& f, void* h, void* const (&planes)[3], cudaStream_
                            : launch_rows<T, 2>(f, h, planes, stream);
 }
 
+// Up to this many features the backward pass computes g and u again (4 D
+// operations per row and hidden unit) instead of reading what the forward
+// pass kept (6 bytes written and read): 25088 x 256 x 1024, fp16 GELU:
+// REGRAD_NOTE
+constexpr int64_t kRecomputeFeatures = 512;
+
 // ------------------------------------------------------------ planning
 struct Extent {
   int64_t m, n;
@@ -330,6 +336,10 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
 template <typename T, int MODE, bool A_MN, bool B_MN>
 int launch_typed(const GemmParams& prm, int bn, int act, cudaStream_t stream) {
   constexpr int kSilu = CCV_ACTIVATION_SILU, kGelu = CCV_ACTIVATION_GELU;
+  if constexpr (MODE == ffn::REGRAD) {
+    return act == kGelu ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
+                        : launch_variant<T, MODE, 256, A_MN, B_MN, kSilu>(prm, stream);
+  }
   if constexpr (MODE != ffn::PLAIN) {
     if (act == kGelu) {
       return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
@@ -407,7 +417,8 @@ struct Product {
     t.m = static_cast<int>(m);
     t.n = static_cast<int>(n);
     t.tiles_m = static_cast<int>(ceil_div(m, 256));
-    t.tiles_n = static_cast<int>(ceil_div(n, MODE == ffn::GATE ? plan.bn / 2 : plan.bn));
+    constexpr bool gated = MODE == ffn::GATE || MODE == ffn::REGRAD;
+    t.tiles_n = static_cast<int>(ceil_div(n, gated ? plan.bn / 2 : plan.bn));
     t.first = static_cast<int>(tiles);
     t.band_inverse = static_cast<uint32_t>((1ULL << 32) / (ffn::kRasterRows * static_cast<uint64_t>(t.tiles_n)));
     tiles += static_cast<int64_t>(t.tiles_m) * t.tiles_n;
@@ -417,7 +428,7 @@ struct Product {
     if (rc != CCV_OK) return rc;
     if (prm.status == nullptr) return CCV_ERR_DEVICE;
     // Fewer problems than planned for leave fewer tiles.
-    prm.whole = static_cast<int>(std::min<int64_t>(plan.whole, tiles));
+    prm.whole = static_cast<int>(MODE == ffn::REGRAD ? tiles : std::min<int64_t>(plan.whole, tiles));
     const int64_t tail = tiles - prm.whole;
     const int64_t units = prm.whole + tail * plan.splits;
     if (units > 0x7fffffff) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
@@ -500,7 +511,9 @@ BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
   const Extent eh = {s.rows, s.hidden}, ex = {s.rows, s.features};
   p.dw_extent[0] = p.dw_extent[1] = {s.hidden, s.features};
   p.dw_extent[2] = {s.features, s.hidden};
-  p.grad = make_plan(&eh, 1, ceil_div(s.features, ffn::kStepK), false, false);
+  p.grad = make_plan(&eh, 1, ceil_div(s.features, ffn::kStepK), false,
+                     ffn_saved_planes(s.features) == 1);
+  if (ffn_saved_planes(s.features) == 1) p.grad.bn = 256;  // REGRAD has one width
   p.dx = make_plan(&ex, 1, 2 * ceil_div(s.hidden, ffn::kStepK), true, false);
   p.dw = make_plan(p.dw_extent, 3, ceil_div(s.rows, ffn::kStepK), true, false);
   p.dg = take_rows(c, s.rows, s.hidden);
@@ -521,6 +534,8 @@ BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
 }
 
 }  // namespace
+
+int ffn_saved_planes(int64_t features) { return features <= kRecomputeFeatures ? 1 : 4; }
 
 size_t ffn_plane_bytes(const FfnShape& s) {
   return static_cast<size_t>(s.rows) * padded(s.hidden) * 2;
@@ -545,10 +560,11 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   const size_t plane = ffn_plane_bytes(s);
   Carver c{static_cast<char*>(ws)};
   const ForwardPlan p = plan_forward(s, saved != nullptr, c);
+  const bool keep = ffn_saved_planes(d) > 1;  // g and u, for the backward pass
   if (m <= kFewRows) {
     void* h = saved != nullptr ? saved : p.h;
     void* planes[3] = {};
-    for (int i = 0; i < 3 && saved != nullptr; ++i) planes[i] = saved + (i + 1) * plane;
+    for (int i = 0; i < 3 && saved != nullptr && keep; ++i) planes[i] = saved + (i + 1) * plane;
     return s.dtype == CCV_DTYPE_BF16 ? run_rows<__nv_bfloat16>(f, h, planes, stream)
                                      : run_rows<__half>(f, h, planes, stream);
   }
@@ -565,7 +581,7 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
     g.operand_b(0, wg.matrix());
     g.operand_b(1, wu.matrix());
     g.result(0, h, m, hid, fp);
-    if (saved != nullptr) {
+    if (saved != nullptr && keep) {
       for (int i = 1; i <= 3; ++i) g.plane(&g.prm.out[i], saved + i * plane, m, hid, fp);
       g.prm.save = 1;
     }
@@ -607,15 +623,31 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
       wd{b.w_down, hid, d, hid, p.w_down};
   RowCopies copies, out_copies;
   dy.fill(copies);
-  if (dw[0] != nullptr || dw[1] != nullptr) x.fill(copies);
+  const bool recompute = ffn_saved_planes(d) == 1;
+  if (recompute || dw[0] != nullptr || dw[1] != nullptr) x.fill(copies);
   if (need_grad) wd.fill(copies);
-  if (b.dx != nullptr) {
+  if (b.dx != nullptr || (need_grad && recompute)) {
     wg.fill(copies);
     wu.fill(copies);
   }
   int rc = copy_rows(copies, stream);
   if (rc != CCV_OK) return rc;
-  if (need_grad) {
+  if (need_grad && recompute) {
+    Product<ffn::REGRAD, false, false> g(s.dtype, p.grad, d, s.activation);
+    g.prm.segments = 2;
+    g.operand_a(0, x.matrix());
+    g.operand_a(1, dy.matrix());
+    g.operand_b(0, wg.matrix());
+    g.operand_b(1, wu.matrix());
+    if (g.rc == CCV_OK) {
+      const Matrix w = wd.matrix();
+      g.rc = encode_2d(&g.prm.b[2], s.dtype, w.base, w.inner, w.outer, w.ld, 64, 64);
+    }
+    g.result(0, p.dg, m, hid, fp);
+    g.result(1, p.du, m, hid, fp);
+    g.problem(0, m, hid);
+    if ((rc = g.launch(stream)) != CCV_OK) return rc;
+  } else if (need_grad) {
     Product<ffn::GRAD, false, true> g(s.dtype, p.grad, d, s.activation);
     g.operand_a(0, dy.matrix());
     g.operand_b(0, wd.matrix());

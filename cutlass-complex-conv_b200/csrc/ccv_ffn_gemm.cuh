@@ -2,7 +2,8 @@
 // kernel template for all of them:
 //   GATE   h = act(x Wg^T) (x Wu^T)        epilogue: activation and product
 //   PLAIN  c = a b (+ a' b')               down projection, dx, weight gradients
-//   GRAD   dh = dy Wd                      epilogue: dg, du from dh, g, u
+//   GRAD   dh = dy Wd                      epilogue: dg, du from dh and the g, u kept
+//   REGRAD g, u as GATE, dh as GRAD        epilogue: dg, du; nothing was kept of g, u
 //
 // A cluster of two CTAs computes a tile of 256 x BN with
 // tcgen05.mma.cta_group::2: each CTA holds 128 rows of A and half of B's BN
@@ -33,7 +34,7 @@
 namespace ccv {
 namespace ffn {
 
-enum Mode { GATE, PLAIN, GRAD };
+enum Mode { GATE, PLAIN, GRAD, REGRAD };
 
 constexpr int kRows = 128;        // rows of one CTA's tile
 constexpr int kStepK = 64;        // reduction elements per pipeline stage: 128-byte rows
@@ -74,7 +75,7 @@ struct Config {
   static constexpr int kStage = kOperandA + kOperandB;
   // The gate epilogue is bound by issue slots and latency: sixteen warps work
   // on a 256-wide tile (39 -> 35 us at 25088 x 256 -> 2 x 1024 GELU).
-  static constexpr int kEpiWarps = MODE == GATE && BN == 256 ? 16 : 8;
+  static constexpr int kEpiWarps = (MODE == GATE || MODE == REGRAD) && BN == 256 ? 16 : 8;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kGroups = kEpiWarps / 4;  // warps that share a row quarter's columns
   // BN = 256: one block per SM.  BN = 128, for problems of few tiles: few
@@ -89,6 +90,8 @@ struct Config {
   static constexpr int kBarOffset = kStagingOffset + kStaging;
   static constexpr int kBarBytes = 512;
   static constexpr int kSmem = kBarOffset + kBarBytes + 1024;
+  // REGRAD: g, u and (BN / 2 columns) dh of one tile, one accumulator.
+  static constexpr int kAccumulators = MODE == REGRAD ? 1 : 2;
   static constexpr int kTmemCols = 2 * BN;
   static_assert(kSmem <= 232448, "shared memory");
   static_assert((2 * kStages + 5 + 2 * kEpiWarps) * 8 + 16 <= kBarBytes, "barriers");
@@ -306,7 +309,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
   if (threadIdx.x == 32) flags[0] = *reinterpret_cast<volatile int*>(p.status) != 0 ? 1 : 0;
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&p.a[0]);
-    ptx::prefetch_tmap(&p.b[MODE == GATE ? rank : 0]);
+    ptx::prefetch_tmap(&p.b[MODE == GATE || MODE == REGRAD ? rank : 0]);
     ptx::prefetch_tmap(&p.out[0]);
   }
   if (warp == 1) {
@@ -335,13 +338,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
       for (int u = cid; u < p.units && !abort; u += ncl) {
         const Unit w = decode(p, u);
         const int m0 = (2 * w.tm + static_cast<int>(rank)) * kRows;
-        const int n0 = MODE == GATE ? w.tn * (BN / 2) : w.tn * BN + static_cast<int>(rank) * (BN / 2);
+        constexpr bool kGated = MODE == GATE || MODE == REGRAD;  // BN / 2 outputs a tile
+        const int n0 = kGated ? w.tn * (BN / 2) : w.tn * BN + static_cast<int>(rank) * (BN / 2);
         for (int seg = 0; seg < p.segments && !abort; ++seg) {
           const int first = max(w.k0 - seg * p.ksteps, 0);
           const int last = min(w.k1 - seg * p.ksteps, p.ksteps);
           const int map = p.problems > 1 ? w.problem : seg;
           const CUtensorMap* ma = &p.a[map];
-          const CUtensorMap* mb = &p.b[MODE == GATE ? static_cast<int>(rank) : map];
+          // REGRAD's second segment is dh: dy with the down projection, whose
+          // hidden index is innermost, half of the tile's outputs per CTA.
+          const bool down = MODE == REGRAD && seg == 1;
+          const CUtensorMap* mb = &p.b[down ? 2 : (kGated ? static_cast<int>(rank) : map)];
           for (int ks = first; ks < last; ++ks) {
             if (!ptx::mbar_wait_bounded(empty_bar(stage), parity, p.status, kTimeoutCode)) {
               flags[1] = 1;
@@ -353,7 +360,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
             const uint32_t sb = sa + kOperandA;
             const int k = ks * kStepK;
             if (issuer) {
-              if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * C::kStage);
+              if (leader) {
+                ptx::mbar_arrive_expect_tx(full_bar(stage),
+                                           2 * (down ? kOperandA + 8192 : C::kStage));
+              }
               if constexpr (A_MN) {
                 ptx::tma_load_2d_pair(sa, ma, fb, m0, k);
                 ptx::tma_load_2d_pair(sa + 8192, ma, fb, m0 + 64, k);
@@ -365,6 +375,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
                 for (int i = 0; i < BN / 128; ++i) {
                   ptx::tma_load_2d_pair(sb + 8192 * i, mb, fb, n0 + 64 * i, k);
                 }
+              } else if (down) {
+                ptx::tma_load_2d_pair(sb, mb, fb, n0 + static_cast<int>(rank) * 64, k);
               } else {
                 ptx::tma_load_2d_pair(sb, mb, fb, k, n0);
               }
@@ -403,8 +415,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
       bool abort = false;
       for (int u = cid; u < p.units && !abort; u += ncl, ++i) {
         const Unit w = decode(p, u);
-        const int buf = i & 1;
-        if (!ptx::mbar_wait_bounded(tempty_bar(buf), ((i >> 1) & 1u) ^ 1u, p.status, kTimeoutCode)) {
+        const int buf = i % C::kAccumulators;
+        if (!ptx::mbar_wait_bounded(tempty_bar(buf), ((i / C::kAccumulators) & 1u) ^ 1u, p.status,
+                                    kTimeoutCode)) {
           flags[1] = 1;
           break;
         }
@@ -419,7 +432,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
           ptx::tc_fence_after();
           const uint64_t da = da0 + stage * (C::kStage / 16);
           const uint64_t db = db0 + stage * (C::kStage / 16);
-          if (issuer) {
+          if (MODE == REGRAD && ks >= p.ksteps) {
+            if (issuer) {
+              constexpr uint32_t down = ptx::idesc_f16(2 * kRows, BN / 2, kIsBf16<T>, false, true);
+              const uint64_t dw =
+                  ptx::desc_mnmajor_sw128(smem_base + kOperandA, 8192) + stage * (C::kStage / 16);
+#pragma unroll
+              for (int kk = 0; kk < kStepK / 16; ++kk) {
+                ptx::mma_f16_pair(d + BN, da + kk * kStepA, dw + kk * (2048 / 16), down,
+                                  (ks != p.ksteps || kk != 0) ? 1u : 0u);
+              }
+              ptx::mma_commit_pair(empty_bar(stage));
+            }
+          } else if (issuer) {
 #pragma unroll
             for (int kk = 0; kk < kStepK / 16; ++kk) {
               ptx::mma_f16_pair(d, da + kk * kStepA, db + kk * kStepB, idesc,
@@ -456,8 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
     for (int u = cid; u < p.units && !skip; u += ncl, ++i) {
       const Unit w = decode(p, u);
       const Tiles& t = p.tiles[w.problem];
-      const int buf = i & 1;
-      const uint32_t use = static_cast<uint32_t>(i >> 1);
+      const int buf = i % C::kAccumulators;
+      const uint32_t use = static_cast<uint32_t>(i / C::kAccumulators);
       const int row0 = (2 * w.tm + static_cast<int>(rank)) * kRows + quarter * 32;
       const bool rows_in = row0 < t.m;
       const uint32_t acc = t_row + static_cast<uint32_t>(buf * BN);
@@ -529,6 +554,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
           put([&](int k) { return high_halves(v[2 * k], v[2 * k + 1]); }, &p.out[2]);
           put([&](int k) { return next_bytes(g[2 * k], v[2 * k], g[2 * k + 1], v[2 * k + 1]); },
               &p.out[3]);
+        }
+      } else if constexpr (MODE == REGRAD) {
+        // 32 outputs per warp, 16 at a time (three values each).
+        const int fc = group * 32;
+        const int col = w.tn * (BN / 2) + fc;
+        const uint32_t dg_slot = ring2.take(lane), du_slot = ring2.take(lane);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t g[16], v[16], d[16];
+          ptx::tmem_ld_32x32b_x16(acc + fc + h * 16, g);
+          ptx::tmem_ld_32x32b_x16(acc + BN / 2 + fc + h * 16, v);
+          ptx::tmem_ld_32x32b_x16(acc + BN + fc + h * 16, d);
+          ptx::tmem_wait_ld();
+          ptx::reg_fence(g);
+          ptx::reg_fence(v);
+          ptx::reg_fence(d);
+          if (h == 1) release();
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t og[4], ou[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = 8 * j + 2 * k;
+              float v0, s0, v1, s1;
+              activation<ACT>(__uint_as_float(g[at]), v0, s0);
+              activation<ACT>(__uint_as_float(g[at + 1]), v1, s1);
+              const float d0 = __uint_as_float(d[at]), d1 = __uint_as_float(d[at + 1]);
+              og[k] = pack2(d0 * __uint_as_float(v[at]) * s0, d1 * __uint_as_float(v[at + 1]) * s1,
+                            T());
+              ou[k] = pack2(d0 * v0, d1 * v1, T());
+            }
+            st_shared_v4(slot64(dg_slot, lane, 2 * h + j), og[0], og[1], og[2], og[3]);
+            st_shared_v4(slot64(du_slot, lane, 2 * h + j), ou[0], ou[1], ou[2], ou[3]);
+          }
+        }
+        publish();
+        if (lane == 0) {
+          if (store && rows_in && col < t.n) {
+            ptx::tma_store_2d(&p.out[0], dg_slot, col, row0);
+            ptx::tma_store_2d(&p.out[1], du_slot, col, row0);
+          }
+          ptx::bulk_commit_group();
+          ptx::bulk_commit_group();  // one group per slot of the ring
         }
       } else if constexpr (MODE == GRAD) {
 #pragma unroll 1
@@ -627,7 +695,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
           }
         }
       }
-      if constexpr (MODE != GATE) release();
+      if constexpr (MODE == PLAIN || MODE == GRAD) release();
       if (!ok) break;
     }
     // Output stores still in flight complete before the CTA exits.

@@ -211,7 +211,7 @@ struct FfnForward {
   int64_t x_stride;
   const void *w_gate, *w_up, *w_down;
   void* y;
-  void* saved;  // four planes for the backward pass (h; g and u to 24 bits), or null
+  void* saved;  // planes for the backward pass (h; unless recomputed, g and u to 24 bits), or null
   // Where a row length is a multiple of 8 elements its matrices are read by
   // TMA in place: bases 16-byte aligned, row strides multiples of 8.
 };
@@ -224,6 +224,8 @@ struct FfnBackward {
   const void *w_gate, *w_up, *w_down, *saved;
   void *dx, *dw_gate, *dw_up, *dw_down;  // each may be null
 };
+// Planes of `saved`: h alone, or h and three that hold g and u.
+int ffn_saved_planes(int64_t features);
 // Bytes of one [rows][hidden] plane (rows padded to 16 bytes).
 size_t ffn_plane_bytes(const FfnShape& s);
 size_t ffn_forward_workspace_bytes(const FfnShape& s, bool save);
