@@ -635,8 +635,8 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
   if (need_grad && recompute) {
     Product<ffn::REGRAD, false, false> g(s.dtype, p.grad, d, s.activation);
     g.prm.segments = 2;
-    g.operand_a(0, x.matrix());
-    g.operand_a(1, dy.matrix());
+    g.operand_a(0, dy.matrix());
+    g.operand_a(1, x.matrix());
     g.operand_b(0, wg.matrix());
     g.operand_b(1, wu.matrix());
     if (g.rc == CCV_OK) {

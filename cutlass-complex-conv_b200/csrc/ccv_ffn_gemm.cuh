@@ -90,7 +90,7 @@ struct Config {
   static constexpr int kBarOffset = kStagingOffset + kStaging;
   static constexpr int kBarBytes = 512;
   static constexpr int kSmem = kBarOffset + kBarBytes + 1024;
-  // REGRAD: g, u and (BN / 2 columns) dh of one tile, one accumulator.
+  // REGRAD: one accumulator of BN columns for g and u, two of BN / 2 for dh.
   static constexpr int kAccumulators = MODE == REGRAD ? 1 : 2;
   static constexpr int kTmemCols = 2 * BN;
   static_assert(kSmem <= 232448, "shared memory");
@@ -345,9 +345,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
           const int last = min(w.k1 - seg * p.ksteps, p.ksteps);
           const int map = p.problems > 1 ? w.problem : seg;
           const CUtensorMap* ma = &p.a[map];
-          // REGRAD's second segment is dh: dy with the down projection, whose
+          // REGRAD's first segment is dh: dy with the down projection, whose
           // hidden index is innermost, half of the tile's outputs per CTA.
-          const bool down = MODE == REGRAD && seg == 1;
+          const bool down = MODE == REGRAD && seg == 0;
           const CUtensorMap* mb = &p.b[down ? 2 : (kGated ? static_cast<int>(rank) : map)];
           for (int ks = first; ks < last; ++ks) {
             if (!ptx::mbar_wait_bounded(empty_bar(stage), parity, p.status, kTimeoutCode)) {
@@ -416,12 +416,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
       for (int u = cid; u < p.units && !abort; u += ncl, ++i) {
         const Unit w = decode(p, u);
         const int buf = i % C::kAccumulators;
-        if (!ptx::mbar_wait_bounded(tempty_bar(buf), ((i / C::kAccumulators) & 1u) ^ 1u, p.status,
-                                    kTimeoutCode)) {
-          flags[1] = 1;
-          break;
-        }
-        ptx::tc_fence_after();
+        auto wait_free = [&]() {
+          const bool free = ptx::mbar_wait_bounded(
+              tempty_bar(buf), ((i / C::kAccumulators) & 1u) ^ 1u, p.status, kTimeoutCode);
+          if (!free) flags[1] = 1;
+          ptx::tc_fence_after();
+          return free;
+        };
+        // REGRAD multiplies dh into the buffer of the tile before last (whose
+        // epilogue was waited for then) while the last tile's is at work, and
+        // waits before g and u.
+        if (MODE != REGRAD && !wait_free()) break;
         const uint32_t d = tmem_base + static_cast<uint32_t>(buf * BN);
         for (int ks = w.k0; ks < w.k1; ++ks) {
           if (!ptx::mbar_wait_bounded(full_bar(stage), parity, p.status, kTimeoutCode)) {
@@ -430,17 +435,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
             break;
           }
           ptx::tc_fence_after();
+          if (MODE == REGRAD && ks == p.ksteps && !wait_free()) {
+            abort = true;
+            break;
+          }
           const uint64_t da = da0 + stage * (C::kStage / 16);
           const uint64_t db = db0 + stage * (C::kStage / 16);
-          if (MODE == REGRAD && ks >= p.ksteps) {
+          if (MODE == REGRAD && ks < p.ksteps) {
             if (issuer) {
               constexpr uint32_t down = ptx::idesc_f16(2 * kRows, BN / 2, kIsBf16<T>, false, true);
               const uint64_t dw =
                   ptx::desc_mnmajor_sw128(smem_base + kOperandA, 8192) + stage * (C::kStage / 16);
 #pragma unroll
               for (int kk = 0; kk < kStepK / 16; ++kk) {
-                ptx::mma_f16_pair(d + BN, da + kk * kStepA, dw + kk * (2048 / 16), down,
-                                  (ks != p.ksteps || kk != 0) ? 1u : 0u);
+                ptx::mma_f16_pair(d + BN + (i & 1) * (BN / 2), da + kk * kStepA,
+                                  dw + kk * (2048 / 16), down, (ks != 0 || kk != 0) ? 1u : 0u);
               }
               ptx::mma_commit_pair(empty_bar(stage));
             }
@@ -448,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
 #pragma unroll
             for (int kk = 0; kk < kStepK / 16; ++kk) {
               ptx::mma_f16_pair(d, da + kk * kStepA, db + kk * kStepB, idesc,
-                                (ks != w.k0 || kk != 0) ? 1u : 0u);
+                                (ks != (MODE == REGRAD ? p.ksteps : w.k0) || kk != 0) ? 1u : 0u);
             }
             ptx::mma_commit_pair(empty_bar(stage));
           }
@@ -565,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Config<MODE, BN>::kT
           uint32_t g[16], v[16], d[16];
           ptx::tmem_ld_32x32b_x16(acc + fc + h * 16, g);
           ptx::tmem_ld_32x32b_x16(acc + BN / 2 + fc + h * 16, v);
-          ptx::tmem_ld_32x32b_x16(acc + BN + fc + h * 16, d);
+          ptx::tmem_ld_32x32b_x16(acc + BN + (i & 1) * (BN / 2) + fc + h * 16, d);
           ptx::tmem_wait_ld();
           ptx::reg_fence(g);
           ptx::reg_fence(v);
