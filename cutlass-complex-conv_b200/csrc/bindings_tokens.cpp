@@ -231,10 +231,11 @@ FfnWeights check_ffn(const torch::Tensor& x, const torch::Tensor& w_gate,
 // Columns of a plane of the saved buffer (rows of whole 16-byte units).
 int64_t saved_width(int64_t hidden) { return (hidden + 7) / 8 * 8; }
 
-// Its planes: what the library asks for one row.
-int64_t saved_planes(int64_t features, int64_t hidden) {
-  return static_cast<int64_t>(ccv_gated_ffn_saved_bytes(1, features, hidden)) /
-         (2 * saved_width(hidden));
+// Its planes: what the library asks for, by the size of one.
+int64_t saved_planes(int64_t rows, int64_t features, int64_t hidden) {
+  rows = rows > 0 ? rows : 1;
+  return static_cast<int64_t>(ccv_gated_ffn_saved_bytes(rows, features, hidden)) /
+         (2 * rows * saved_width(hidden));
 }
 
 int activation_code(const std::string& name) {
@@ -258,7 +259,7 @@ std::tuple<torch::Tensor, torch::Tensor> gated_ffn_forward(torch::Tensor x, torc
   size_t saved_bytes = 0;
   if (save) {
     saved_bytes = ccv_gated_ffn_saved_bytes(r.rows, r.features, w.hidden);
-    saved = fresh({saved_planes(r.features, w.hidden), r.rows, saved_width(w.hidden)},
+    saved = fresh({saved_planes(r.rows, r.features, w.hidden), r.rows, saved_width(w.hidden)},
                   x.scalar_type(), x);
   }
   const size_t bytes = ccv_gated_ffn_forward_workspace_bytes(r.rows, r.features, w.hidden, save);
@@ -287,7 +288,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn
   check_like(saved, x, "saved");
   const Rows rx = as_tma_rows(x), rdy = as_tma_rows(dy);
   TORCH_CHECK_VALUE(saved.scalar_type() == x.scalar_type() && saved.is_contiguous() &&
-                        saved.dim() == 3 && saved.size(0) == saved_planes(rx.features, w.hidden) && saved.size(1) == rx.rows &&
+                        saved.dim() == 3 && saved.size(0) == saved_planes(rx.rows, rx.features, w.hidden) && saved.size(1) == rx.rows &&
                         saved.size(2) == saved_width(w.hidden),
                     "saved must be what the forward call returned for these shapes");
   torch::Tensor dx, dg, du, dd;

@@ -5,10 +5,10 @@
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // with x [M, D], Wg and Wu [F, D], Wd [D, F].  h, dg and du are rounded to the
 // operands' type once each: they are operands of the next product, whose
-// inputs the tensor cores take in 16 bits.  g and u are kept for the backward
-// pass to 24 bits.
+// inputs the tensor cores take in 16 bits.  g and u are computed again in the
+// backward pass, or (many features) kept for it to 24 bits.
 //
-// Forward: GATE, PLAIN.  Backward: GRAD, PLAIN over two segments (dx), PLAIN
+// Forward: GATE, PLAIN.  Backward: GRAD or REGRAD, PLAIN over two segments (dx), PLAIN
 // over three problems in one launch (the weight gradients).  This file plans
 // the tiles, builds the tensor maps and launches ccv_ffn_gemm.cuh's kernel.
 //
@@ -214,8 +214,12 @@ int run_rows(const FfnForward& f, void* h, void* const (&planes)[3], cudaStream_
 
 // Up to this many features the backward pass computes g and u again (4 D
 // operations per row and hidden unit) instead of reading what the forward
-// pass kept (6 bytes written and read): 25088 x 256 x 1024, fp16 GELU:
-// REGRAD_NOTE
+// pass kept (6 bytes written and read), which also takes a quarter of the
+// memory.  Both passes together, kept against computed again, bf16 SiLU:
+// 25088 x 256 x 1024 182 / 155 us, 25088 x 384 x 1024 230 / 216, 12544 x 512 x
+// 2048 258 / 252, 8192 x 768 x 3200 334 / 346, 8192 x 1024 x 4096 504 / 549.
+// Not where there are fewer than two waves of tiles: there the doubled chain
+// of K steps is what counts (600 x 360 x 704 backward 22.5 / 24.7).
 constexpr int64_t kRecomputeFeatures = 512;
 
 // ------------------------------------------------------------ planning
@@ -512,8 +516,8 @@ BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
   p.dw_extent[0] = p.dw_extent[1] = {s.hidden, s.features};
   p.dw_extent[2] = {s.features, s.hidden};
   p.grad = make_plan(&eh, 1, ceil_div(s.features, ffn::kStepK), false,
-                     ffn_saved_planes(s.features) == 1);
-  if (ffn_saved_planes(s.features) == 1) p.grad.bn = 256;  // REGRAD has one width
+                     ffn_saved_planes(s) == 1);
+  if (ffn_saved_planes(s) == 1) p.grad.bn = 256;  // REGRAD has one width
   p.dx = make_plan(&ex, 1, 2 * ceil_div(s.hidden, ffn::kStepK), true, false);
   p.dw = make_plan(p.dw_extent, 3, ceil_div(s.rows, ffn::kStepK), true, false);
   p.dg = take_rows(c, s.rows, s.hidden);
@@ -535,7 +539,10 @@ BackwardPlan plan_backward(const FfnShape& s, Carver& c) {
 
 }  // namespace
 
-int ffn_saved_planes(int64_t features) { return features <= kRecomputeFeatures ? 1 : 4; }
+int ffn_saved_planes(const FfnShape& s) {
+  const int64_t tiles = ceil_div(s.rows, 256) * ceil_div(s.hidden, 128);
+  return s.features <= kRecomputeFeatures && tiles >= device_sm_count() ? 1 : 4;
+}
 
 size_t ffn_plane_bytes(const FfnShape& s) {
   return static_cast<size_t>(s.rows) * padded(s.hidden) * 2;
@@ -560,7 +567,7 @@ int launch_ffn_forward(const FfnForward& f, void* ws, cudaStream_t stream) {
   const size_t plane = ffn_plane_bytes(s);
   Carver c{static_cast<char*>(ws)};
   const ForwardPlan p = plan_forward(s, saved != nullptr, c);
-  const bool keep = ffn_saved_planes(d) > 1;  // g and u, for the backward pass
+  const bool keep = ffn_saved_planes(s) > 1;  // g and u, for the backward pass
   if (m <= kFewRows) {
     void* h = saved != nullptr ? saved : p.h;
     void* planes[3] = {};
@@ -623,7 +630,7 @@ int launch_ffn_backward(const FfnBackward& b, void* ws, cudaStream_t stream) {
       wd{b.w_down, hid, d, hid, p.w_down};
   RowCopies copies, out_copies;
   dy.fill(copies);
-  const bool recompute = ffn_saved_planes(d) == 1;
+  const bool recompute = ffn_saved_planes(s) == 1;
   if (recompute || dw[0] != nullptr || dw[1] != nullptr) x.fill(copies);
   if (need_grad) wd.fill(copies);
   if (b.dx != nullptr || (need_grad && recompute)) {

@@ -193,7 +193,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// g and u for the backward pass, to 24 bits of float32 each (a relative step
+// g and u kept for the backward pass, to 24 bits of float32 each (a relative step
 // of 2^-15; 16 bits of either would show in dx and in the weight gradients
 // beside the roundings of dg and of the result): planes of the high 16 bits
 // of g, of u, and of the next 8 bits of both (g's in the low byte).

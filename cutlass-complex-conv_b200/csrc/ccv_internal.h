@@ -225,7 +225,7 @@ struct FfnBackward {
   void *dx, *dw_gate, *dw_up, *dw_down;  // each may be null
 };
 // Planes of `saved`: h alone, or h and three that hold g and u.
-int ffn_saved_planes(int64_t features);
+int ffn_saved_planes(const FfnShape& s);
 // Bytes of one [rows][hidden] plane (rows padded to 16 bytes).
 size_t ffn_plane_bytes(const FfnShape& s);
 size_t ffn_forward_workspace_bytes(const FfnShape& s, bool save);

@@ -174,7 +174,7 @@ int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, 
 size_t ccv_gated_ffn_saved_bytes(int64_t rows, int64_t features, int64_t hidden) {
   const FfnShape s = {rows, features, hidden, CCV_DTYPE_BF16, 0};
   return guarded_size(
-      [&]() -> size_t { return check_ffn(s) == CCV_OK ? ffn_saved_planes(features) * ffn_plane_bytes(s) : 0; });
+      [&]() -> size_t { return check_ffn(s) == CCV_OK ? ffn_saved_planes(s) * ffn_plane_bytes(s) : 0; });
 }
 
 size_t ccv_gated_ffn_forward_workspace_bytes(int64_t rows, int64_t features, int64_t hidden,
@@ -214,7 +214,7 @@ int ccv_gated_ffn_forward(const void* x, int64_t x_row_stride, const void* w_gat
         (rc = check_in_place(y, features, 0, "y must be 16-byte aligned")) != CCV_OK) {
       return rc;
     }
-    if (saved != nullptr && (!aligned_to(saved, 256) || saved_bytes < ffn_saved_planes(features) * ffn_plane_bytes(f.shape))) {
+    if (saved != nullptr && (!aligned_to(saved, 256) || saved_bytes < ffn_saved_planes(f.shape) * ffn_plane_bytes(f.shape))) {
       return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");
     }
     if ((rc = check_workspace(workspace, workspace_bytes,
@@ -269,7 +269,7 @@ int ccv_gated_ffn_backward(const void* dy, int64_t dy_row_stride, const void* x,
     if ((rc = check_in_place(dw_down, hidden, 0, "gradients must be 16-byte aligned")) != CCV_OK) {
       return rc;
     }
-    if (rows > 0 && (!aligned_to(saved, 256) || saved_bytes < ffn_saved_planes(features) * ffn_plane_bytes(b.shape))) {
+    if (rows > 0 && (!aligned_to(saved, 256) || saved_bytes < ffn_saved_planes(b.shape) * ffn_plane_bytes(b.shape))) {
       return set_error(CCV_ERR_WORKSPACE, "saved buffer misaligned or too small");
     }
     if ((rc = check_workspace(workspace, workspace_bytes,
