@@ -172,7 +172,8 @@ def test_autograd_of_parts():
             assert torch.equal(t.grad, want) if n else t.grad is None
 
 
-@pytest.mark.parametrize("rows, features, hidden", [(7, 256, 512), (3000, 256, 512)])
+@pytest.mark.parametrize("rows, features, hidden", [(7, 256, 512), (3000, 256, 512),
+                                                    (20000, 128, 520), (5000, 520, 1032)])
 def test_same_result_every_time_and_on_another_stream(rows, features, hidden):
     x, wg, wu, wd, dy = _inputs(rows, features, hidden)
 
