@@ -32,7 +32,7 @@ CU_SOURCES = ["ccv_api.cu", "ccv_fprop.cu", "ccv_fprop2.cu", "ccv_fprop2h.cu", "
               "ccv_noalloc.cu", "ccv_backward.cu", "ccv_norm.cu", "ccv_ffn.cu", "ccv_dropout.cu",
               "ccv_tokens_api.cu"]
 CU_HEADERS = ["ccv_internal.h", "ccv_ptx.cuh", "ccv_fprop_common.cuh", "ccv_epilogue.cuh",
-              "ccv_layout_role.cuh", "ccv_tokens.cuh",
+              "ccv_layout_role.cuh", "ccv_tokens.cuh", "ccv_norm_shift.h",
               "ccv_ffn_gemm.cuh", "ccv_ffn_rows.cuh"]
 EXT_SOURCES = ["bindings.cpp", "bindings_tokens.cpp"]
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

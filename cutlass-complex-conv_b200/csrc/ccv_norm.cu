@@ -25,13 +25,15 @@
 // group's rows are then a multiple of V rows apart, so they all start at the
 // same one, and the group's vectors are shifted by it; the first and the last
 // may hold elements of the row's neighbours, which a bit mask excludes
-// (SHIFT).  Other layouts take single elements, and rows wider than 8192 the
-// kernels further down.
+// (SHIFT).  Other layouts, and rows shorter than the vectors would reach past
+// them, take single elements, and rows wider than 8192 the kernels further
+// down.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
 
 #include "ccv_internal.h"
+#include "ccv_norm_shift.h"
 #include "ccv_ptx.cuh"
 #include "ccv_tokens.cuh"
 
@@ -211,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per_block = blockDim.x / g;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  const int shift = SHIFT ? static_cast<int>((first + group) * features % V) : 0;
-  auto column = [&](int i) { return (i * g + lane) * V - shift; };
+  const int shift = SHIFT ? shift_of_row(first + group, features, V) : 0;
+  auto column = [&](int i) { return shifted_column(i, g, lane, V, shift); };
   Inside<V> inside;
   if (SHIFT) {
 #pragma unroll
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int c = column(i);
-        if (SHIFT && r == rows - 1 && c + V > features) {
+        if (SHIFT && past_the_end(r, rows, c, features, V)) {
           Hx::fetch_end(at, i, row, c, features);
         } else if (c < features) {
           Hx::fetch(at, i, row, c);
@@ -351,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per_block = blockDim.x / g;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block;
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
-  const int shift = SHIFT ? static_cast<int>((first + group) * features % V) : 0;
-  auto column = [&](int i) { return (i * g + lane) * V - shift; };
+  const int shift = SHIFT ? shift_of_row(first + group, features, V) : 0;
+  auto column = [&](int i) { return shifted_column(i, g, lane, V, shift); };
   const uint32_t ring_base = ptx::smem_u32(ring);
   const uint32_t x_bytes = blockDim.x * Hx::kBytes;
   const uint32_t stage_bytes = x_bytes + blockDim.x * Hy::kBytes;
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const int c = column(i);
-          if (SHIFT && r == rows - 1 && c + V > features) {
+          if (SHIFT && past_the_end(r, rows, c, features, V)) {
             Hx::fetch_end(at, i, xr, c, features);
             Hy::fetch_end(at + x_bytes, i, gr, c, features);
           } else if (c < features) {
@@ -793,7 +795,7 @@ Rings plan_rings(int64_t rows, int g, int v) {
 // Whether rows of `n` dense elements can be read as shifted vectors of V.
 template <typename T, int V>
 bool shifted_rows(const void* p, int64_t stride, int64_t n) {
-  return stride == n && vec_rows<T, V>(p, 0, V);
+  return shift_fits(n, V) && stride == n && vec_rows<T, V>(p, 0, V);
 }
 
 unsigned row_blocks(int64_t rows) {
