@@ -13,6 +13,9 @@ asynchronous on the current stream and differentiable; the ``*_backward``
 functions are the gradients themselves, for callers that keep their own tape.
 """
 
+import collections
+import weakref
+
 import torch
 from torch import nn
 
@@ -207,22 +210,131 @@ class GatedFeedForward(nn.Module):
         return f"{self.features}, {self.hidden}, activation={self.activation!r}"
 
 
-class Dropout(nn.Module):
-    """``dropout`` that counts its own calls: each forward in training mode
-    takes the next ``offset``.  In evaluation mode ``x`` passes (with
-    ``residual`` added, if given)."""
+_CALLS_KEPT = 4096
+# Keys of masks drawn from torch's seed, away from keys that callers choose.
+_DRAWN = 0x9E3779B97F4A7C15
 
-    def __init__(self, p=0.1, seed=0):
+
+class _Call:
+    """A call of a Dropout module that a backward pass may have to repeat."""
+
+    __slots__ = "number", "node", "repeated"
+
+    def __init__(self, number):
+        self.number, self.node, self.repeated = number, None, False
+
+    def over(self):
+        """Whether nothing can ask for it any more: its graph is gone or, for
+        a call that recorded none (reentrant checkpointing), it was repeated."""
+        return self.repeated if self.node is None else self.node() is None
+
+
+class _Calls(collections.OrderedDict):
+    """A module's last calls, by the generator's state each began at:
+    {state: [_Call]}.  Copies and pickles of a module start without any."""
+
+    def __reduce__(self):
+        return _Calls, ()
+
+
+def _generator_state(device):
+    """State of torch's generator for ``device``, which it moves on by one
+    step; None while the current stream is captured (its state is on the
+    device then)."""
+    if device.type != "cuda":
+        return device.type, 0, int(torch.randint(1 << 62, ()))
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    generator = torch.cuda.default_generators[device.index]
+    state = device.index, generator.initial_seed(), generator.get_offset()
+    generator.set_offset(state[2] + 4)  # torch counts in fours
+    return state
+
+
+class Dropout(nn.Module):
+    """``dropout`` with a new mask at each call in training mode.  In
+    evaluation mode ``x`` passes (with ``residual`` added, if given).
+
+    Without ``seed`` the masks are a function of torch's generator for x's
+    device, as ``torch.nn.Dropout``'s are: each call moves it on, so modules
+    draw different masks, processes seeded differently do too, and a saved
+    generator state resumes the sequence.  With ``seed`` call n draws mask
+    ``(seed, n)``, whatever the generator's seed: give each module and each
+    process its own.  The count is in ``state_dict``.
+
+    A call that activation checkpointing repeats draws its mask again: it
+    finds the generator in the state it had then.  Where it does not
+    (``preserve_rng_state=False``) the repetition raises ``RuntimeError``.  In
+    a captured graph the offset is drawn on the device, so that each replay
+    has new masks.  ``offset`` in the call (an int, or a tensor as in
+    ``dropout``) replaces all that, and nothing is counted."""
+
+    def __init__(self, p=0.1, seed=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be between 0 and 1, got {p}")
         self.p, self.seed, self.calls = p, seed, 0
+        self._begun = _Calls()
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, offset=None):
         if not self.training or self.p == 0.0:
             return x if residual is None else residual + x
-        offset, self.calls = self.calls, self.calls + 1
-        return dropout(x, self.p, self.seed, offset, residual)
+        seed = _DRAWN if self.seed is None else self.seed
+        if offset is not None:
+            return dropout(x, self.p, seed, offset, residual)
+        state = _generator_state(x.device)
+        repeated = torch._C._current_graph_task_id() != -1  # inside a backward pass
+        if state is None:
+            if repeated:
+                self._refuse("a stream is being captured")
+            offset = torch.randint(1 << 62, (1,), device=x.device)
+            return dropout(x, self.p, seed, offset, residual)
+        call = self._repeated(state) if repeated else self._new(state)
+        offset = call.number
+        if self.seed is None:
+            seed, offset = state[1] ^ _DRAWN, state[2]
+        y = dropout(x, self.p, seed, offset, residual)
+        if not repeated and y.grad_fn is not None:
+            call.node = weakref.ref(y.grad_fn)
+        return y
+
+    def _new(self, state):
+        call = _Call(self.calls)
+        self.calls += 1
+        before = self._begun.pop(state, None)
+        self._begun[state] = [call] if before is None else [c for c in before if not c.over()] + [call]
+        if len(self._begun) > _CALLS_KEPT:
+            self._begun.popitem(last=False)
+        return call
+
+    def _repeated(self, state):
+        calls = self._begun.get(state, [])
+        calls = [c for c in calls if c.node is None or not c.over()] or calls
+        if not calls:
+            self._refuse("the generator is in no state that a forward call began at")
+        if len(calls) > 1 and self.seed is not None:
+            self._refuse("several calls began at this state of the generator")
+        calls[-1].repeated = True
+        return calls[-1]
+
+    def _refuse(self, why):
+        raise RuntimeError(
+            f"Dropout was called inside a backward pass and cannot tell which call's mask to "
+            f"repeat ({why}): pass offset=, or checkpoint with preserve_rng_state=True")
+
+    def get_extra_state(self):
+        return torch.tensor(self.calls)
+
+    def set_extra_state(self, state):
+        self.calls = int(state)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+        key = prefix + "_extra_state"
+        if key in missing_keys:  # saved before the count was kept
+            missing_keys.remove(key)
 
     def extra_repr(self):
         return f"p={self.p}, seed={self.seed}"
