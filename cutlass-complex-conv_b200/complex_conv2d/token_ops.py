@@ -128,6 +128,14 @@ def _dropout(x, p, seed, offset, residual):
     return _C.dropout(x, p, seed & _U64, offset & _U64, None, residual)
 
 
+def _dropout_backward(dy, p, seed, offset, x_dtype):
+    if dy.dtype == x_dtype:  # the same call on the gradient
+        return _dropout(dy, p, seed, offset, None)
+    if isinstance(offset, torch.Tensor):
+        return _C.dropout_backward(dy, p, seed & _U64, 0, offset, x_dtype)
+    return _C.dropout_backward(dy, p, seed & _U64, offset & _U64, None, x_dtype)
+
+
 class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset):
@@ -142,7 +150,7 @@ class _DropoutFunction(torch.autograd.Function):
     def backward(ctx, dy):
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = _dropout(dy, ctx.p, ctx.seed, ctx.offset, None).to(ctx.x_dtype)
+            dx = _dropout_backward(dy, ctx.p, ctx.seed, ctx.offset, ctx.x_dtype)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 

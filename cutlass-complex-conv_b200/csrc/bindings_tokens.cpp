@@ -308,6 +308,14 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> gated_ffn
   return {dx, dg, du, dd};
 }
 
+const int64_t* check_offset(const OptTensor& offset, const torch::Tensor& x) {
+  if (!given(offset)) return nullptr;
+  check_like(*offset, x, "offset");
+  TORCH_CHECK_TYPE(offset->scalar_type() == at::kLong, "offset must be an int64 tensor");
+  TORCH_CHECK_VALUE(offset->numel() == 1, "offset must have one element");
+  return offset->data_ptr<int64_t>();
+}
+
 torch::Tensor dropout(torch::Tensor x, double p, uint64_t seed, uint64_t offset,
                       OptTensor offset_device, OptTensor residual) {
   check_cuda(x, "x");
@@ -324,13 +332,7 @@ torch::Tensor dropout(torch::Tensor x, double p, uint64_t seed, uint64_t offset,
   const int yt = dtype_code(out, "residual");
   TORCH_CHECK_TYPE(xt == CCV_DTYPE_F32 || yt == CCV_DTYPE_F32 || yt == xt,
                    "residual must be float32 or of the 16-bit input's type");
-  const int64_t* od = nullptr;
-  if (given(offset_device)) {
-    check_like(*offset_device, x, "offset");
-    TORCH_CHECK_TYPE(offset_device->scalar_type() == at::kLong, "offset must be an int64 tensor");
-    TORCH_CHECK_VALUE(offset_device->numel() == 1, "offset must have one element");
-    od = offset_device->data_ptr<int64_t>();
-  }
+  const int64_t* od = check_offset(offset_device, x);
   c10::cuda::CUDAGuard guard(x.device());
   auto xc = x.contiguous();
   auto y = fresh(x.sizes(), out, x);
@@ -338,6 +340,24 @@ torch::Tensor dropout(torch::Tensor x, double p, uint64_t seed, uint64_t offset,
                        current_stream()),
            "ccv_dropout");
   return y;
+}
+
+torch::Tensor dropout_backward(torch::Tensor dy, double p, uint64_t seed, uint64_t offset,
+                               OptTensor offset_device, at::ScalarType x_dtype) {
+  check_cuda(dy, "dy");
+  const int yt = dtype_code(dy.scalar_type(), "dy");
+  const int xt = dtype_code(x_dtype, "x_dtype");
+  TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "p must be between 0 and 1, got ", p);
+  TORCH_CHECK_TYPE(xt == CCV_DTYPE_F32 || yt == CCV_DTYPE_F32 || yt == xt,
+                   "dy must be float32 or of the 16-bit input's type");
+  const int64_t* od = check_offset(offset_device, dy);
+  c10::cuda::CUDAGuard guard(dy.device());
+  auto g = dy.contiguous();
+  auto dx = fresh(dy.sizes(), x_dtype, dy);
+  check_rc(ccv_dropout_backward(g.data_ptr(), yt, dx.data_ptr(), xt, dy.numel(), p, seed, offset, od,
+                                current_stream()),
+           "ccv_dropout_backward");
+  return dx;
 }
 
 }  // namespace
@@ -360,4 +380,6 @@ void register_token_operators(pybind11::module_& m) {
         py::arg("need_dup"), py::arg("need_ddown"));
   m.def("dropout", &dropout, "counter-based dropout", py::arg("x"), py::arg("p"),
         py::arg("seed"), py::arg("offset"), py::arg("offset_device"), py::arg("residual"));
+  m.def("dropout_backward", &dropout_backward, "-> dx", py::arg("dy"), py::arg("p"),
+        py::arg("seed"), py::arg("offset"), py::arg("offset_device"), py::arg("x_dtype"));
 }

@@ -238,7 +238,7 @@ struct Dropout {
   const void* residual;  // may be null; of y's type
   void* y;
   int64_t count;
-  int x_dtype, y_dtype;
+  int x_dtype, y_dtype;  // one type, or at least one of them fp32
   double p;
   uint64_t seed, offset;
   const int64_t* offset_dev;  // overrides offset when not null

@@ -99,6 +99,27 @@ int check_workspace(const void* ws, size_t have, size_t need) {
   return CCV_OK;
 }
 
+// Checks of both dropout entries and the launch; `types`: what to say of two
+// 16-bit types that differ.
+int run_dropout(const Dropout& a, const char* types, ccv_stream_t stream) {
+  if (!valid_dtype(a.x_dtype) || !valid_dtype(a.y_dtype)) return invalid("unknown element type");
+  if (a.count < 0) return invalid("count must be non-negative");
+  if (a.count > kMaxElements) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
+  if (!(a.p >= 0.0 && a.p <= 1.0)) return invalid("p must be between 0 and 1");
+  if (a.x_dtype != CCV_DTYPE_F32 && a.y_dtype != CCV_DTYPE_F32 && a.y_dtype != a.x_dtype) {
+    return invalid(types);
+  }
+  if (a.count == 0) return CCV_OK;
+  if (a.x == nullptr || a.y == nullptr) return invalid("null tensor pointer");
+  if (!aligned_to(a.x, dtype_bytes(a.x_dtype)) || !aligned_to(a.y, dtype_bytes(a.y_dtype)) ||
+      !aligned_to(a.residual, dtype_bytes(a.y_dtype)) || !aligned_to(a.offset_dev, 8)) {
+    return invalid("tensor pointers must be aligned to their element");
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int rc = begin_launches(st);
+  return rc != CCV_OK ? rc : launch_dropout(a, st);
+}
+
 }  // namespace
 }  // namespace ccv
 
@@ -286,27 +307,20 @@ int ccv_dropout(const void* x, int x_dtype, const void* residual, void* y, int y
                 int64_t count, double p, uint64_t seed, uint64_t offset,
                 const int64_t* offset_device, ccv_stream_t stream) {
   return guarded([&]() -> int {
-    if (!valid_dtype(x_dtype) || !valid_dtype(y_dtype)) return invalid("unknown element type");
-    if (count < 0) return invalid("count must be non-negative");
-    if (count > kMaxElements) return set_error(CCV_ERR_UNSUPPORTED, "tensor too large");
-    if (!(p >= 0.0 && p <= 1.0)) return invalid("p must be between 0 and 1");
-    if (residual == nullptr && y_dtype != x_dtype) {
+    if (valid_dtype(x_dtype) && valid_dtype(y_dtype) && residual == nullptr && y_dtype != x_dtype) {
       return invalid("without a residual the output has the input's type");
     }
-    if (x_dtype != CCV_DTYPE_F32 && y_dtype != CCV_DTYPE_F32 && y_dtype != x_dtype) {
-      return invalid("a 16-bit input takes a residual of its own type or float32");
-    }
-    if (count == 0) return CCV_OK;
-    if (x == nullptr || y == nullptr) return invalid("null tensor pointer");
-    if (!aligned_to(x, dtype_bytes(x_dtype)) || !aligned_to(y, dtype_bytes(y_dtype)) ||
-        !aligned_to(residual, dtype_bytes(y_dtype)) || !aligned_to(offset_device, 8)) {
-      return invalid("tensor pointers must be aligned to their element");
-    }
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const int rc = begin_launches(st);
-    if (rc != CCV_OK) return rc;
-    Dropout a = {x, residual, y, count, x_dtype, y_dtype, p, seed, offset, offset_device};
-    return launch_dropout(a, st);
+    return run_dropout({x, residual, y, count, x_dtype, y_dtype, p, seed, offset, offset_device},
+                       "a 16-bit input takes a residual of its own type or float32", stream);
+  });
+}
+
+int ccv_dropout_backward(const void* dy, int y_dtype, void* dx, int x_dtype, int64_t count,
+                         double p, uint64_t seed, uint64_t offset, const int64_t* offset_device,
+                         ccv_stream_t stream) {
+  return guarded([&]() -> int {
+    return run_dropout({dy, nullptr, dx, count, y_dtype, x_dtype, p, seed, offset, offset_device},
+                       "the gradient of a 16-bit input is of its own type or float32", stream);
   });
 }
 

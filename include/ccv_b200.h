@@ -326,6 +326,12 @@ int ccv_dropout(const void* x, int x_dtype, const void* residual, void* y, int y
                 int64_t count, double p, uint64_t seed, uint64_t offset,
                 const int64_t* offset_device, ccv_stream_t stream);
 
+/* Gradient of ccv_dropout's x where a residual gave y another type: dx (of
+ * x's type) from dy (of y's), multiplied in fp32 and rounded once. */
+int ccv_dropout_backward(const void* dy, int y_dtype, void* dx, int x_dtype, int64_t count,
+                         double p, uint64_t seed, uint64_t offset, const int64_t* offset_device,
+                         ccv_stream_t stream);
+
 /* Device status word of the current device: nonzero after an in-kernel
  * bounded wait ran out (a CCV_ERR_* code).  While it is set, fprop kernels
  * on that device exit without work.  The kernel that gives up also writes a
