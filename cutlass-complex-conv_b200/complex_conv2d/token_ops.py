@@ -20,6 +20,7 @@ import torch
 from torch import nn
 
 from ._extension import cutlass_complex_conv as _C
+from ._tangents import refuse_tangents
 
 __all__ = [
     "layer_norm", "layer_norm_with_stats", "layer_norm_backward",
@@ -55,6 +56,7 @@ class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_tangents("the gradient of layer_norm", dy)
         x, mean, rstd, weight = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dw, db = _C.layer_norm_backward(dy, x, mean, rstd, weight, ctx.bias_dtype, need[0],
@@ -71,6 +73,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     float32 from a 16-bit input, or for any of the three from float32 (so
     float32 planes can feed a 16-bit block without a copy).
     """
+    refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFunction.apply(x, weight, bias, eps, out_dtype)
@@ -102,6 +105,7 @@ class _GatedFeedForwardFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_tangents("the gradient of gated_feed_forward", dy)
         need = ctx.needs_input_grad
         return (*_C.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation, need[0], need[1],
                                        need[2], need[3]), None)
@@ -116,6 +120,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     cores' operand types; sums are in float32).  ``activation``: ``"silu"`` or
     ``"gelu"`` (the exact form with erf).
     """
+    refuse_tangents("gated_feed_forward", x, w_gate, w_up, w_down)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):
         return _GatedFeedForwardFunction.apply(x, w_gate, w_up, w_down, activation)
     return _C.gated_ffn_forward(x, w_gate, w_up, w_down, activation, False)[0]
@@ -148,6 +153,7 @@ class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        refuse_tangents("the gradient of dropout", dy)
         dx = None
         if ctx.needs_input_grad[0]:
             dx = _dropout_backward(dy, ctx.p, ctx.seed, ctx.offset, ctx.x_dtype)
@@ -167,6 +173,7 @@ def dropout(x, p, seed, offset=0, residual=None):
     a new mask on each replay after its owner has changed it.  Use another
     offset for each call of a step.
     """
+    refuse_tangents("dropout", x, residual)
     if torch.is_grad_enabled() and (
             x.requires_grad or (residual is not None and residual.requires_grad)):
         return _DropoutFunction.apply(x, residual, p, seed, offset)
