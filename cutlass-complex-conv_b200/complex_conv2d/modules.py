@@ -24,6 +24,7 @@ import torch
 from torch import nn
 
 from ._extension import cutlass_complex_conv
+from ._tangents import refuse_tangents
 
 _PRECISIONS = {"tf32": 0, "3xtf32": 1}
 # Input bytes per chunk in the middle of forward_host's pipeline.
@@ -101,6 +102,7 @@ class _ComplexConv2dFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        refuse_tangents("the gradient of ComplexConv2d", dy)
         (x,) = ctx.saved_tensors
         m = ctx.module
         dy = dy.contiguous()
@@ -132,6 +134,7 @@ class _ComplexConv2dPlanarFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy_real, dy_imag):
+        refuse_tangents("the gradient of ComplexConv2d", dy_real, dy_imag)
         x_real, x_imag = ctx.saved_tensors
         m = ctx.module
         dy_real = dy_real.contiguous()
@@ -347,6 +350,8 @@ class ComplexConv2d(nn.Module):
         Returns:
             ``[y_real, y_imag]`` as contiguous NHWC float32 tensors.
         """
+        refuse_tangents("ComplexConv2d", x_real, x_imag, self.weight_real, self.weight_imag,
+                        self.bias_real, self.bias_imag)
         if torch.is_grad_enabled() and (
             x_real.requires_grad
             or x_imag.requires_grad
@@ -426,6 +431,8 @@ class ComplexConv2d(nn.Module):
                 "input and ComplexConv2d weights must be on the same CUDA device"
             )
 
+        refuse_tangents("ComplexConv2d", x, self.weight_real, self.weight_imag, self.bias_real,
+                        self.bias_imag)
         if torch.is_grad_enabled() and (
             x.requires_grad
             or self.weight_real.requires_grad
