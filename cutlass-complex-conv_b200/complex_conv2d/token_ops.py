@@ -293,7 +293,8 @@ class Dropout(nn.Module):
 
     def forward(self, x, residual=None, offset=None):
         if not self.training or self.p == 0.0:
-            return x if residual is None else residual + x
+            # (The sum of two types is float32: rounded to the residual's, as in training.)
+            return x if residual is None else (residual + x).to(residual.dtype)
         seed = _DRAWN if self.seed is None else self.seed
         if offset is not None:
             return dropout(x, self.p, seed, offset, residual)
