@@ -340,18 +340,19 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
 template <typename T, int MODE, bool A_MN, bool B_MN>
 int launch_typed(const GemmParams& prm, int bn, int act, cudaStream_t stream) {
   constexpr int kSilu = CCV_ACTIVATION_SILU, kGelu = CCV_ACTIVATION_GELU;
-  if constexpr (MODE == ffn::REGRAD) {
+  if constexpr (MODE == ffn::REGRAD) {  // of one width
     return act == kGelu ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
                         : launch_variant<T, MODE, 256, A_MN, B_MN, kSilu>(prm, stream);
-  }
-  if constexpr (MODE != ffn::PLAIN) {
-    if (act == kGelu) {
-      return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
-                       : launch_variant<T, MODE, 128, A_MN, B_MN, kGelu>(prm, stream);
+  } else {
+    if constexpr (MODE != ffn::PLAIN) {
+      if (act == kGelu) {
+        return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kGelu>(prm, stream)
+                         : launch_variant<T, MODE, 128, A_MN, B_MN, kGelu>(prm, stream);
+      }
     }
+    return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kSilu>(prm, stream)
+                     : launch_variant<T, MODE, 128, A_MN, B_MN, kSilu>(prm, stream);
   }
-  return bn == 256 ? launch_variant<T, MODE, 256, A_MN, B_MN, kSilu>(prm, stream)
-                   : launch_variant<T, MODE, 128, A_MN, B_MN, kSilu>(prm, stream);
 }
 
 template <int MODE, bool A_MN, bool B_MN>
