@@ -92,7 +92,7 @@ int copy_rows(const RowCopies& c, cudaStream_t stream) {
   if (c.count == 0) return CCV_OK;
   int64_t most = 1;
   for (int i = 0; i < c.count; ++i) most = std::max(most, c.m[i].rows);
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((most + 7) / 8, 148 * 8));
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((most + 7) / 8, device_sm_count() * 8));
   return launched(
       launch_kernel(ffn_copy_rows, dim3(blocks, c.count), dim3(256), 0, stream, 1, c), "row copy");
 }
@@ -319,7 +319,7 @@ int launch_variant(const GemmParams& prm, cudaStream_t stream) {
     err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (err != cudaSuccess) return;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(4 * 148, 1, 1);
+    cfg.gridDim = dim3(4 * device_sm_count(), 1, 1);
     cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     int n = 0;

@@ -800,7 +800,7 @@ bool shifted_rows(const void* p, int64_t stride, int64_t n) {
 
 unsigned row_blocks(int64_t rows) {
   const int64_t blocks = (rows + 7) / 8;
-  return static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8);
+  return static_cast<unsigned>(std::min<int64_t>(blocks, device_sm_count() * 8));
 }
 
 template <typename Tx, typename Tw, typename Ty, int V, int VPT>
