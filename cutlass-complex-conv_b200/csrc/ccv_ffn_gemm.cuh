@@ -166,10 +166,14 @@ __device__ __forceinline__ float rcp(float x) {
 }
 
 // act(g) and act'(g).  The sigmoid is two hardware approximations (2^x and
-// 1/x, a few 2^-23 each).  GELU's normal distribution is Abramowitz and
-// Stegun 7.1.26 (|error of erf| <= 1.5e-7), a polynomial times exp(-g^2/2),
-// the exponential its slope needs too.  Both errors, and the flush of values
-// below 2^-126 to zero, lie far below the 16-bit rounding of the result.
+// 1/x, a few 2^-23 each): a relative error far below the 16-bit rounding of
+// the result.  GELU's normal distribution is Abramowitz and Stegun 7.1.26, a
+// polynomial times exp(-g^2/2), the exponential its slope needs too.  Its
+// bound is an absolute one (|error of erf| <= 1.5e-7, and a few 2^-24), so in
+// the lower tail the relative error passes the result's rounding: 1.9e-4 at
+// g = -3.5, 4.7e-4 at -4 (half a step of float16 is 4.9e-4, of bfloat16
+// 3.9e-3), 1.6e-3 at -5, 3.6e-3 at -6, of values from 8e-4 down.  (A float32
+// 1 + erf(g / sqrt 2) loses more to cancellation from -5 on.)
 template <int ACT>
 __device__ __forceinline__ void activation(float g, float& value, float& slope) {
   if constexpr (ACT == CCV_ACTIVATION_SILU) {
