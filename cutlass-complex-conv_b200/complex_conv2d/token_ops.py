@@ -258,7 +258,7 @@ def _generator_state(device):
     step; None while the current stream is captured (its state is on the
     device then)."""
     if device.type != "cuda":
-        return device.type, 0, int(torch.randint(1 << 62, ()))
+        return device.type, 0, int(torch.randint(1 << 62, (), device=device))
     if torch.cuda.is_current_stream_capturing():
         return None
     generator = torch.cuda.default_generators[device.index]
@@ -340,7 +340,7 @@ class Dropout(nn.Module):
             f"repeat ({why}): pass offset=, or checkpoint with preserve_rng_state=True")
 
     def get_extra_state(self):
-        return torch.tensor(self.calls)
+        return torch.tensor(self.calls, device="cpu")
 
     def set_extra_state(self, state):
         self.calls = int(state)

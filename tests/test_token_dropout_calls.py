@@ -188,6 +188,37 @@ def test_a_resumed_run_continues_the_sequence(device):
     net.load_state_dict({k: v for k, v in net.state_dict().items() if "0." in k}, strict=True)
 
 
+def test_count_is_kept_on_the_host_whatever_the_default_device():
+    """A state made or loaded under another default device."""
+    a, b = cc.Dropout(0.5, 4), cc.Dropout(0.5, 4)
+    a.calls = 7
+    with torch.device("meta"):
+        state = a.state_dict()
+        b.load_state_dict(state)
+    assert b.calls == 7
+
+
+@pytest.mark.parametrize("seed", [None, 4])
+@pytest.mark.parametrize("inner", [False, True])
+@pytest.mark.parametrize("outer", [False, True])
+def test_nested_segments(device, outer, inner, seed):
+    d = cc.Dropout(0.5, seed)
+    x = _x(device)
+    seen = []
+
+    def step(t):
+        seen.append(t)
+        return d(t).square()
+
+    grad, y = _gradient(lambda t: checkpoint(
+        lambda u: checkpoint(step, step(u), use_reentrant=inner) + u, t, use_reentrant=outer), x)
+    # y = x + (2 (2 x)^2)^2 where both masks kept it: dy/dx = 1 + 4 (y - x) / x.
+    want = 1 + 4 * (y.double() - x.double()) / x.double()
+    assert len(seen) > 3  # how often is the checkpointing's affair
+    assert torch.equal(grad == 1, y == x)
+    torch.testing.assert_close(grad.double(), want, rtol=1e-4, atol=1e-4)
+
+
 def test_memory_of_calls_is_bounded(device):
     d = cc.Dropout(0.5, 4)
     x = _x(device, 1)
