@@ -11,7 +11,8 @@
 // is stored.  Bound by memory with a
 // residual (51 M elements, bf16 plus fp32: 80-84 us, 6.2-6.4 TB/s, 96-99 % of
 // the copy rate on B200) and nearly so by the generator's issue slots without
-// (25 M bf16: 19 us, 5.3 TB/s).
+// (25 M bf16: 19 us, 5.3 TB/s).  A gradient from one type to another, 51 M
+// elements through autograd: fp32 to bf16 53 us, bf16 to fp32 64 us (308 MB).
 #include <cmath>
 
 #include "ccv_internal.h"

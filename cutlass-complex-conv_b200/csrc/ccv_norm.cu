@@ -18,7 +18,7 @@
 // rows there, reading nothing twice; blocks leave fp32 partial sums that a
 // second launch adds in block order (deterministic).  Measured on B200, 200704
 // x 256, fp32 x, bf16 y: forward 49.9 us (6.2 TB/s, 96 % of the copy rate),
-// backward 86-89 us (5.8-6.0 TB/s); bf16 12545 x 1024 13.6 and 22 us.
+// backward 86-90 us (5.7-6.0 TB/s); bf16 12545 x 1024 13.6 and 22 us.
 //
 // Rows that 16-byte vectors do not divide go in pairs of elements where those
 // divide them.  Dense rows of odd width start at any element of a vector: a
