@@ -119,7 +119,7 @@ def gated_feed_forward(x, w_gate, w_up, w_down, activation="silu"):
     ``w_down [features, hidden]``, all bfloat16 or all float16 (the tensor
     cores' operand types; sums are in float32, and the hidden values between
     the products are rounded to the type, so in float16 they must stay within
-    65504).  ``activation``: ``"silu"`` or ``"gelu"`` (the exact form with erf).
+    65504 and lose bits below 6e-5, in the gradients too).  ``activation``: ``"silu"`` or ``"gelu"`` (the exact form with erf).
     """
     refuse_tangents("gated_feed_forward", x, w_gate, w_up, w_down)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down)):

@@ -288,7 +288,7 @@ int ccv_layer_norm_backward(const void* dy, int y_dtype, int64_t dy_row_stride, 
  * filled with what the backward pass reads (an opaque layout).  The
  * intermediate rows h = act(g) u, and the gradients of g and u, are rounded to
  * the type once each, as operands of the next product: in fp16 a value
- * beyond 65504 becomes infinite there.  Where features (x, w_gate, w_up, y and their gradients) or
+ * beyond 65504 becomes infinite there, and one below 6e-5 loses bits.  Where features (x, w_gate, w_up, y and their gradients) or
  * hidden (w_down and its gradient) is a multiple of 8, those matrices are
  * read and written in place by TMA: 16-byte aligned bases, row strides
  * multiples of 8.  Others are copied to padded rows in the workspace.
